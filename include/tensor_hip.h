@@ -1,7 +1,7 @@
 /*
  * libtensor_hip.so — the ROCm (gfx950) provider's C ABI.
  *
- * Two groups of entry points:
+ * Three groups of entry points:
  *
  *  1. GGUF quantized-linear kernels, in the reference's native entry shape
  *     TensorKernelV1 (src/tensor/include/tensor/abi.h:135-141).  Each validates
@@ -16,7 +16,9 @@
  *      benchmarks/kernels/showcase/benchmark.py:276-290,
  *      src/tensor/providers/cuda/device.py:211-229).
  *
- *  2. Runtime services the Python provider binds through ctypes, replacing the
+ *  2. The paged-cache operators (slot maps, rotary positions, attention), in the same shape.
+ *
+ *  3. Runtime services the Python provider binds through ctypes, replacing the
  *     CUDA driver calls of src/tensor/providers/cuda/driver.py:40-145
  *     (memory, copies, streams, events, graphs, device properties).
  *
@@ -266,6 +268,87 @@ int32_t tensor_gguf_gemv_swiglu_v1(const TensorCallV1 *call, TensorErrorV1 *erro
  *   2 type scalar uint32 GGML type id
  */
 int32_t tensor_gguf_dequant_v1(const TensorCallV1 *call, TensorErrorV1 *error);
+
+/* ------------------------------------------- paged cache and attention ---
+ *
+ * The operators between a layer's q + k + v linears and its output linear, on a key/value cache
+ * kept in pages.  No counterpart in the reference, whose model inference is elsewhere.  A cache is
+ * two fp16 buffers [pages, kv_heads, page_size, dim], page_size a power of two from 1 to 1024.  A
+ * slot is page * page_size + place in the page.  A request's own tokens fill the pages of its table
+ * row in order; tokens that all requests share (a common prompt) may stand before them, in pages of
+ * a list of their own.  Lengths, counts, tables and lists are read on the device: a captured graph
+ * follows them as they grow.  int32 buffers need 4-byte alignment, the others 16.
+ */
+
+/*
+ * One step's block tables and slot map from the requests' lengths.  Request b holds lengths[b] tokens
+ * of its own and adds counts[b]; pages it lacks come off the end of the free list, in request order.
+ * Arguments, in order:
+ *    0 lengths     int32 [B]     tokens held (negative: as 0)
+ *    1 counts      int32 [B]     new tokens (negative: as 0)
+ *    2 start       int32 [1]     position of a request's first own token (the shared prefix's length)
+ *    3 free        int32 [F]     free pages, a stack: the last of the first free_count goes first
+ *    4 free_count  int32 [1]
+ *    5 table       int32 [B, P]  page of each page_size tokens of a request, -1 past its last
+ *    6 T           scalar int32  rows of the token outputs, at least the sum of counts
+ *    7 offsets     int32 [B + 1] out: first row of each request's tokens, then their number
+ *    8 lengths_out int32 [B]     out: lengths + counts
+ *    9 positions   int32 [T]     out: start + place in the request; -1 past the last token
+ *   10 slots       int32 [T]     out: slot; -1 past the last token and for a token without a page
+ *   11 table_out   int32 [B, P]  out: the table with the new pages
+ *   12 free_left   int32 [1]     out: free_count less the pages taken; negative: so many were missing,
+ *                                 and the entries that lack one are -1
+ *   13 page_size   scalar uint32
+ */
+int32_t tensor_paged_slots_v1(const TensorCallV1 *call, TensorErrorV1 *error);
+
+/*
+ * Rotary positions: the pair (a, b) of dimensions becomes (a c - b s, b c + a s), c and s the row of the
+ * token's position in `angles`; dimensions past `rotated` are copied.  Pairs are (p, p + rotated / 2)
+ * (layout 0) or (2 p, 2 p + 1) (layout 1).  inverse = 1 turns back, which is also the gradient of the
+ * forward call.  A token of negative position (padding) gives zeros, one past the table NaN.
+ *    0 q         fp16 or fp32 [T, heads, dim]        4 q_out  as q
+ *    1 k         same dtype [T, kv_heads, dim]       5 k_out  as k
+ *    2 positions int32 [T]                           6 layout scalar uint32
+ *    3 angles    fp32 [reach, rotated]: rotated / 2 cosines, then as many sines    7 inverse scalar uint32
+ */
+int32_t tensor_rotary_v1(const TensorCallV1 *call, TensorErrorV1 *error);
+
+/*
+ * tensor_rotary_v1's forward call with the rotated keys and the values written to the cache at their
+ * slots, each rounded once to fp16.  A slot that is negative or past the cache stores nothing; two tokens
+ * of one slot are the caller's error.
+ *    0 q, 1 k, 2 v  fp16 or fp32 (one dtype) [T, heads, dim], [T, kv_heads, dim], [T, kv_heads, dim]
+ *    3 positions int32 [T]    4 slots int32 [T]    5 angles fp32 [reach, rotated]
+ *    6 q_out fp16 [T, heads, dim]    7 k_cache, 8 v_cache: updated in place    9 layout scalar uint32
+ */
+int32_t tensor_rotary_store_v1(const TensorCallV1 *call, TensorErrorV1 *error);
+
+/*
+ * Attention of every request's new tokens (the last counts of its lengths) over the shared prefix and its
+ * own pages, causal within them: out[t, h] = sum_j softmax_j(scale q[t, h] . k[j]) v[j] over the prefix's
+ * keys and the own keys up to the token's place.  Query head h reads key head h / (heads / kv_heads).  One
+ * token or many for each request, in any mix.  The prefix is read once for the whole batch.  Scores, sums
+ * and outputs are kept in fp32; the softmax weights enter the second product as fp16.  A token that sees
+ * no key gives zeros, and so does a row of q past the last request.  A table entry that is no page of the
+ * cache hides its keys.
+ *    0 q             fp16 [T, heads, dim], dim 64 or 128
+ *    1 k_cache, 2 v_cache  fp16 [pages, kv_heads, page_size, dim]
+ *    3 offsets       int32 [B + 1]  first row of each request's tokens (B up to 1024)
+ *    4 lengths       int32 [B]      own keys, the new tokens' among them
+ *    5 table         int32 [B, P]
+ *    6 prefix_pages  int32 [PP]     pages of the prefix
+ *    7 prefix_length int32 [1]      its keys (0: none)
+ *    8 workspace     uint8 [bytes]  256-byte aligned device scratch, clobbered; at least what
+ *                                   tensor_paged_attention_workspace_v1 tells; not for two calls at once
+ *    9 out           fp16 [T, heads, dim]
+ *   10 scale         scalar fp32, 0 for 1 / sqrt(dim)
+ */
+int32_t tensor_paged_attention_v1(const TensorCallV1 *call, TensorErrorV1 *error);
+
+/* Bytes of workspace tensor_paged_attention_v1 needs for these extents. */
+int32_t tensor_paged_attention_workspace_v1(int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads,
+                                            int64_t dim, uint64_t *bytes, TensorErrorV1 *error);
 
 /* ---------------------------------------------------- runtime services --- */
 

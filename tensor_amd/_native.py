@@ -29,6 +29,10 @@ KERNELS = (
     "tensor_gguf_gemv_variant_v1",
     "tensor_gguf_gemv_q8_1_v1",
     "tensor_gguf_dequant_v1",
+    "tensor_paged_slots_v1",
+    "tensor_rotary_v1",
+    "tensor_rotary_store_v1",
+    "tensor_paged_attention_v1",
 )
 
 _u64, _i32, _f32p = c.c_uint64, c.c_int32, c.POINTER(c.c_float)
@@ -91,6 +95,7 @@ SERVICES = {
     "tensor_gguf_gemm_tile_v1": [_i32, c.POINTER(_i32), c.POINTER(_i32), c.POINTER(_i32)],
     "tensor_gguf_gemv_plan_v1": [c.c_uint32, c.c_int64, c.c_int64, c.c_int64, c.POINTER(_i32), c.POINTER(_i32),
                                  c.POINTER(_i32)],
+    "tensor_paged_attention_workspace_v1": [c.c_int64, c.c_int64, c.c_int64, c.c_int64, c.c_int64, c.POINTER(_u64)],
 }
 
 

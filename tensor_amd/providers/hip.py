@@ -7,8 +7,9 @@ through the TensorCallV1 descriptor and records events.  Every device call goes
 through libtensor_hip.so (include/tensor_hip.h): the kernels are its
 TensorKernelV1 entry points and memory/streams/events are its runtime services.
 
-Executables are the library's built-in GGUF kernels, loaded by name
-(``device.load("gguf_linear", encoding="q4_k")``) or from a manifest dict.
+Executables are the library's built-in kernels, loaded by name
+(``device.load("gguf_linear", encoding="q4_k")``, ``device.load("paged_attention")``) or from a
+manifest dict.
 """
 
 from __future__ import annotations
@@ -322,13 +323,13 @@ class Device(Session):
 
     # -------------------------------------------------------- executables --
     def load(self, artifact, **options) -> Executable:
-        """Load an executable: a built-in GGUF kernel by name (with its options) or manifest
+        """Load an executable: a built-in kernel by name (with its options) or manifest
         dict, or a `hip` executable bundle from a path (a hand-built code object; see
         tensor_amd.artifacts), as the reference's ``Device.load(artifact)`` does for its
         bundles (src/tensor/providers/cuda/device.py:359-386)."""
         import os
 
-        from tensor_amd.gguf.kernels import manifest as gguf_manifest
+        from tensor_amd.kernels.builtin import manifest as builtin_manifest
 
         self._check()
         if isinstance(artifact, os.PathLike) or (isinstance(artifact, str) and os.path.isfile(artifact)):
@@ -336,7 +337,7 @@ class Device(Session):
                 raise ValueError("options apply only to kernels loaded by name")
             return self._load_bundle(artifact)
         if isinstance(artifact, str):
-            manifest = gguf_manifest(artifact, **options)
+            manifest = builtin_manifest(artifact, **options)
         elif isinstance(artifact, dict):
             if options:
                 raise ValueError("options apply only to kernels loaded by name")
@@ -469,6 +470,13 @@ class Device(Session):
         _native.call("tensor_gguf_gemm_plan_v1", ggml_type(encoding), int(m), int(k), (c.c_int64 * len(rows))(*rows),
                      len(rows), int(workspace_bytes), c.byref(tile), c.byref(splits), c.byref(pipelined))
         return dict(gemm_tiles()[tile.value], tile=tile.value, splits=splits.value, pipelined=bool(pipelined.value))
+
+    def attention_workspace(self, tokens: int, requests: int, heads: int, kv_heads: int, dim: int) -> int:
+        """Bytes of workspace a ``paged_attention`` call of these extents needs."""
+        result = c.c_uint64()
+        _native.call("tensor_paged_attention_workspace_v1", int(tokens), int(requests), int(heads), int(kv_heads),
+                     int(dim), c.byref(result))
+        return result.value
 
     def graph(self, callback, *, resources=()):
         """Capture the launches ``callback()`` enqueues into a replayable graph.  The buffers of

@@ -23,11 +23,13 @@ __all__ = ["Kernel", "close", "hip_runtimes", "load"]
 
 
 def load(artifact, **options) -> Kernel:
-    """A registered Kernel for a built-in GGUF kernel name (with its options), a manifest
-    dict or a ``hip`` bundle path.  Module references (``module::export``) need the
+    """A registered Kernel for a built-in kernel name (with its options), a manifest
+    dict or a ``hip`` bundle path; a kernel that updates its inputs (``rotary_store``) is not
+    registered as a functional operator and runs through ``raw`` and ``prepare``.  Module references (``module::export``) need the
     reference's module registry and are refused."""
     if isinstance(artifact, str) and "::" in artifact:
         raise ValueError("module references are not supported; load a kernel name or a hip bundle")
     kernel = Kernel(artifact, **options)
-    kernel.register()
+    if not kernel.mutable_inputs:
+        kernel.register()
     return kernel

@@ -7,12 +7,13 @@ registration.py:10-73: ``metadata`` / ``fake`` / ``raw`` / ``prepare`` /
 torch.compile traces it with symbolic shapes; ``into`` is the registered
 mutation form that writes caller-owned outputs.
 
-Artifacts are the HIP provider's: a built-in GGUF kernel by name with its
+Artifacts are the HIP provider's: a built-in kernel by name with its
 options (``Kernel("gguf_linear", encoding="q4_k")``), a manifest dict, or a
 ``hip`` bundle by path.  Input buffers must be read-only in the kernel and
 declared outputs completely written, never aliasing inputs (the functional
 custom-operator contract); ``mutable_inputs`` names input buffers a kernel
-without declared outputs writes, which ``raw`` and ``prepare`` launch.
+without declared outputs writes, which ``raw`` and ``prepare`` launch (a
+built-in kernel's manifest names its own).
 """
 
 from __future__ import annotations
@@ -45,9 +46,9 @@ def _read_manifest(artifact, options):
         manifest, _ = read_artifact(path)  # every member verified
         return manifest, path.read_bytes(), str(path)
     if isinstance(artifact, str):
-        from tensor_amd.gguf.kernels import manifest as gguf_manifest
+        from tensor_amd.kernels.builtin import manifest as builtin_manifest
 
-        manifest = gguf_manifest(artifact, **options)
+        manifest = builtin_manifest(artifact, **options)
         return manifest, json.dumps(manifest, sort_keys=True).encode(), manifest
     if isinstance(artifact, dict):
         if options:
@@ -65,6 +66,7 @@ class Kernel:
         if self.manifest.get("provider") != "hip":
             raise ValueError("tensor_amd.torch runs HIP provider artifacts")
         names = self.manifest.get("outputs", [])
+        mutable_inputs = mutable_inputs or self.manifest.get("mutable_inputs", ())
         if not names and not mutable_inputs:
             raise ValueError("functional kernels need declared outputs")
         constants = self.manifest.get("constants", {})
