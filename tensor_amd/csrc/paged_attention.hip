@@ -7,6 +7,8 @@
 // are (the sum over keys takes them in any order, V^T's operand in the same).  K and V tiles go to LDS by
 // DMA, V^T comes out of it by transposing reads; chunks of 16 bytes are swizzled by row so that both reads
 // spread over the banks.
+#include <type_traits>
+
 #include "gguf_common.h"
 #include "paged_launch.h"
 #include "paged_plan.h"
@@ -14,7 +16,10 @@
 namespace tensor_paged {
 namespace {
 
+using tensor_gguf::dot2;
+using tensor_gguf::float2_t;
 using tensor_gguf::float4_t;
+using tensor_gguf::half2_t;
 using tensor_gguf::half2_from_fp32;
 using tensor_gguf::half8_t;
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
@@ -24,23 +29,19 @@ constexpr int kThreads = 64 * kWaves;
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// threadIdx.x as a value of its own: what a segment derives from it is then not kept in registers outside
+__device__ __forceinline__ int here() {
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  return tid;
+}
+
 __host__ __device__ inline Extents extents_of(const AttentionArgs& a) {
   return extents(a.tokens, a.requests, a.heads, a.kv, a.page_shift, a.columns, a.prefix_columns);
 }
 __device__ inline Request request_of(const AttentionArgs& a, const Extents& e, int b) {
   return b == a.requests ? prefix_request(e, a.offsets[b], *a.prefix_length)
                          : own_request(e, a.offsets[b], a.offsets[b + 1], a.lengths[b]);
-}
-
-__device__ const uint4 zeros[1] = {};
-
-// 16 bytes a lane from global memory to LDS, lane l to dst + 16 l (dst the same in the whole wave).
-// Written as assembly: the compiler makes every LDS read wait for all such loads in flight, of
-// other buffers too; the waits here are written out where a stage is read.  (Nothing else here uses m0.)
-__device__ __forceinline__ void dma16(const void* src, const void* dst) {
-  const uint32_t at = (uint32_t)(uintptr_t)(const void __attribute__((address_space(3)))*)dst;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               :: "s"(uniform((int)at)), "v"(src) : "memory");
 }
 
 __device__ __forceinline__ half4_t read_transposed(const _Float16* p) {
@@ -60,39 +61,108 @@ __device__ __forceinline__ int key_chunk(int row, int c) { return c ^ (row & (D 
 template <int D>
 __device__ __forceinline__ int value_chunk(int row, int c) { return c ^ (2 * (row & (D / 16 - 1))); }
 
+// Loads of these values are waited for here, where no tile is on its way: the compiler, which does not know
+// of those, waits for all loads before a value's first use.
+template <int N>
+__device__ __forceinline__ void settle(half8_t (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
+}
+
 constexpr float kInfinity = __builtin_inff();
+
+// Maximum over a lane and the one 32 away, and over those 16 apart: rows of lanes of two copies are exchanged.
+// (Assembly, with the wait states a lane exchange needs after a vector write: the compiler takes the two
+// results of its builtin for equal here.)
+__device__ __forceinline__ float max32(float v) {
+  float a = v, b = v;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float max16(float v) {
+  float a = v, b = v;
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  return fmaxf(a, b);
+}
 // The running maximum is raised (and the sums rescaled) only where a score passes it by this many
 // powers of two: weights stay below 2^8 in fp16, and most tiles rescale nothing.
 constexpr float kLazy = 8.0f;
 
+__device__ const uint4 zeros[1] = {};
+
+// 16 bytes a lane from global memory to LDS, lane l to dst + 16 l (dst the same in the whole wave).
+// Written as assembly: the compiler makes every LDS read wait for all such loads in flight, of
+// other buffers too; the waits here are written out where a stage is read.  (Nothing else here uses m0.)
+__device__ __forceinline__ void dma16(const void* src, const void* dst) {
+  const uint32_t at = (uint32_t)(uintptr_t)(const void __attribute__((address_space(3)))*)dst;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :: "s"(uniform((int)at)), "v"(src) : "memory");
+}
+
+__device__ __forceinline__ void dma4(const void* src, const void* dst) {
+  const uint32_t at = (uint32_t)(uintptr_t)(const void __attribute__((address_space(3)))*)dst;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+               :: "s"(uniform((int)at)), "v"(src) : "memory");
+}
+// 16 bytes with the part of the address that a wave shares in scalar registers.
+__device__ __forceinline__ void dma16(const void* base, uint32_t offset, const void* dst) {
+  const uint32_t at = (uint32_t)(uintptr_t)(const void __attribute__((address_space(3)))*)dst;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :: "s"(uniform((int)at)), "v"(offset), "s"(base) : "memory");
+}
+
 // One key head of the cache behind a page list.  A wave holds a window of 64 entries of the list, one in
-// each lane, so that a lookup is a lane exchange and the list's loads are rare.
+// each lane; the next window is on its way to LDS (`ring`, 128 entries of this wave) by then.
 template <int D>
 struct Keys {
   const _Float16 *k, *v;
   const int32_t* list;
-  int pages, kv, head, shift, bound;  // bound: keys past it are not there
-  int first, window, ahead;           // list entry of lane 0, this lane's page (-1: none), the next window's
-  __device__ Keys(const AttentionArgs& a, int head, const int32_t* list, int bound)
-      : k(static_cast<const _Float16*>(a.k_cache)), v(static_cast<const _Float16*>(a.v_cache)), list(list), pages(a.pages),
-        kv(a.kv), head(head), shift(a.page_shift), bound(bound) {}
-  __device__ __forceinline__ int entry(int index) const {
-    const int p = ((int64_t)index << shift) < bound ? list[index] : -1;
-    return (unsigned)p < (unsigned)pages ? p : -1;  // an entry that is no page of the cache hides its keys
+  int32_t* ring;
+  int pages, kv, head, shift, bound;  // keys from bound on are not there
+  int lane;
+  int first, window, flip;            // list entry of lane 0, this lane's page (-1: none), the window's half of the ring
+  uint64_t there;                     // lanes that have a page
+  __device__ Keys(const AttentionArgs& a, int head, const int32_t* list, int bound, int32_t* ring, int lane)
+      : k(static_cast<const _Float16*>(a.k_cache)), v(static_cast<const _Float16*>(a.v_cache)), list(list), ring(ring),
+        pages(a.pages), kv(a.kv), head(head), shift(a.page_shift), bound(bound), lane(lane) {}
+  __device__ __forceinline__ int last() const { return max(bound - 1, 0) >> shift; }
+  __device__ __forceinline__ int valid(int index, int page) const {
+    return index <= last() && (unsigned)page < (unsigned)pages ? page : -1;  // no page of the cache: hides its keys
+  }
+  __device__ __forceinline__ int entry(int index) const { return valid(index, list[min(index, last())]); }
+  __device__ __forceinline__ void fetch(int from, int half) const {
+    dma4(list + min(from + lane, last()), ring + 64 * half);
+  }
+  __device__ __forceinline__ void open() {
+    window = valid(first + lane, ring[64 * flip + lane]);
+    there = __ballot(window >= 0);
   }
   // windows from the one of key `from` on, a tile's first: a tile's entries are in one window
   __device__ __forceinline__ void begin(int from) {
     first = from >> shift;
-    window = entry(first + (int)(threadIdx.x & 63));
-    ahead = entry(first + 64 + (int)(threadIdx.x & 63));
+    flip = 0;
+    fetch(first, 0);
+    fetch(first + 64, 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    open();
   }
+  // (the window opened here was fetched before tiles that have been waited for since)
   __device__ __forceinline__ void reach(int from) {
     if (from >> shift < first + 64) return;
     first += 64;
-    window = ahead;
-    ahead = entry(first + 64 + (int)(threadIdx.x & 63));
+    flip ^= 1;
+    open();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    fetch(first + 64, flip ^ 1);
   }
-  // the page of a key within the window, -1 for none
+  // whether keys [from, from + COUNT), a tile of the window, are all there
+  template <int COUNT>
+  __device__ __forceinline__ bool whole(int from) const {
+    const int entries = COUNT >> shift > 1 ? COUNT >> shift : 1;  // at most 64
+    const uint64_t want = (entries == 64 ? 0 : 1ull << entries) - 1;
+    return from + COUNT <= bound && !(want & ~(there >> ((from >> shift) - first)));
+  }
+  // the page of a key of the window, -1 for none
   __device__ __forceinline__ int page(int key) const {
     const int p = __shfl(window, (key >> shift) - first);
     return key < bound ? p : -1;
@@ -101,30 +171,53 @@ struct Keys {
   __device__ __forceinline__ size_t at(int page, int key) const {
     return ((((size_t)(unsigned)page * kv + head) << shift) + (key & ((1 << shift) - 1))) * D;
   }
+  // byte offset of a key that is there, the same in the whole wave
+  __device__ __forceinline__ size_t row(int key) const {
+    return 2 * at(__builtin_amdgcn_readlane(window, (key >> shift) - first), key);
+  }
 };
 
-// The softmax of one tile of scores against the running maximum: s becomes the weights; returns
-// whether the sums have to be scaled by alpha.
-template <int N>
-__device__ __forceinline__ bool weights(float* s, float top, float& m, float& l, float& alpha, float c) {
-  bool raise = (top - m) * c > kLazy || (m == -kInfinity && top > -kInfinity);
-  alpha = 1.0f;
-  const bool any = __any(raise);
-  if (any) {
-    const float next = fmaxf(m, top);
-    alpha = m == -kInfinity ? 0.0f : exp2f((m - next) * c);
-    m = next;
-    l *= alpha;
-  }
-  const float mc = m == -kInfinity ? 0.0f : m * c;
-  float sum = 0.0f;
+// This wave's rows of a tile: N loads of RPI rows each.  Whole tiles whose loads stay in one page have
+// their rows' offsets in scalar registers; others look each row up, and read zeros for a key that is not there.
+template <int D, int COUNT, int N>
+struct Rows {
+  static constexpr int CH = D / 8, RPI = 512 / D;
+  size_t at[N];
+  bool fast;
+  __device__ __forceinline__ void find(const Keys<D>& keys, int from, int r0) {
+    fast = (1 << keys.shift) >= RPI && keys.template whole<COUNT>(from);
+    if (fast) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    s[i] = __builtin_amdgcn_exp2f(s[i] * c - mc);
-    sum += s[i];
+      for (int n = 0; n < N; ++n) at[n] = keys.row(from + r0 + n * RPI);
+    }
   }
-  l += sum;
-  return any;
+  // lane_at: where a lane's 16 bytes are from the first of its load's rows
+  __device__ __forceinline__ void load(const Keys<D>& keys, int from, int r0, const _Float16* matrix,
+                                       const uint32_t (&lane_at)[N], _Float16* dst) const {
+    const int lane = keys.lane;
+    if (fast) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        dma16(reinterpret_cast<const uint8_t*>(matrix) + at[n], lane_at[n], dst + (r0 + n * RPI) * D);
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int key = from + r0 + n * RPI + lane / CH, p = keys.page(key);
+        const uint32_t chunk = lane_at[n] / 2 - (lane / CH) * D;
+        dma16(p < 0 ? (const void*)zeros : matrix + keys.at(p, key) + chunk, dst + (r0 + n * RPI) * D);
+      }
+    }
+  }
+};
+
+// Moves a row's running maximum m up to `top` where that passes it by 2^kLazy; true if the wave's sums have
+// to be scaled by alpha.
+__device__ __forceinline__ bool raise(float top, float& m, float& alpha, float c) {
+  if (!__any((top - m) * c > kLazy || (m == -kInfinity && top > -kInfinity))) return false;
+  const float next = fmaxf(m, top);
+  alpha = m == -kInfinity ? 0.0f : exp2f((m - next) * c);
+  m = next;
+  return true;
 }
 
 // Where some rows of a tile do not see a key, its weight of 0 would still turn a value that is not
@@ -161,11 +254,11 @@ __device__ __forceinline__ half8_t pack8(const float* s) {
 // One segment of a wide item: up to 128 rows, 32 a wave, against key tiles [t0, t1).
 template <int D>
 __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Extents& x, const Request& r, const Segment& seg,
-                                             const int32_t* pages, float* slot, bool whole, _Float16* lds) {
+                                             const int32_t* pages, float* slot, bool whole, _Float16* lds, int32_t* ring) {
   constexpr int CH = D / 8, RPW = kWideKeys / kWaves, RPI = 512 / D, N = RPW / RPI;
   constexpr int MAT = kWideKeys * D;  // values of one staged matrix
   constexpr int DB = D / 32, AHEAD = 4;
-  const int lane = threadIdx.x & 63, wr = uniform(threadIdx.x >> 6);
+  const int tid = here(), lane = tid & 63, wr = uniform(tid >> 6);
   const int half = lane >> 5;
   const int row = wr * 32 + (lane & 31), ti = row / x.share, j = row - ti * x.share, i = seg.tile * x.per + ti;
   const bool live = ti < x.per && i < r.count;
@@ -184,120 +277,188 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) q[kk] = *reinterpret_cast<const half8_t*>(src + 16 * kk + 8 * half);
   }
-  Keys<D> keys(a, seg.head, pages, bound);
-
-  // this wave's 16 rows of a tile, K and V, to LDS (a key that is not there: zeros); returns which of the
-  // tile's 64 keys are there
-  auto stage = [&](int t, _Float16* dst) {
-    const int from = t * kWideKeys;
-    keys.reach(from);
+  Keys<D> keys(a, seg.head, pages, bound, ring, lane);
+  using Tile = Rows<D, kWideKeys, N>;
+  const int r0 = wr * RPW;  // this wave loads 16 rows of a tile
+  uint32_t k_lane[N], v_lane[N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int r0 = wr * RPW + n * RPI, kr = r0 + lane / CH, p = keys.page(from + kr);
-      const size_t at = keys.at(p, from + kr);
-      dma16(p < 0 ? (const void*)zeros : keys.k + at + 8 * key_chunk<D>(kr, lane % CH), dst + r0 * D);
-      dma16(p < 0 ? (const void*)zeros : keys.v + at + 8 * value_chunk<D>(kr, lane % CH), dst + MAT + r0 * D);
-    }
-    return __ballot(keys.page(from + lane) >= 0);
-  };
+  for (int n = 0; n < N; ++n) {
+    const int kr = r0 + n * RPI + lane / CH;
+    k_lane[n] = 2 * ((lane / CH) * D + 8 * key_chunk<D>(kr, lane % CH));
+    v_lane[n] = 2 * ((lane / CH) * D + 8 * value_chunk<D>(kr, lane % CH));
+  }
   float16_t o[DB] = {};
-  float m = -kInfinity, l = 0.0f;
+  float m = -kInfinity, l = 0.0f, top;
+  float s[16];  // scores, lane: row lane % 32, keys 8 (e / 4) + 4 half + e % 4
 
-  auto compute = [&](int t, uint64_t seen, const _Float16* ks) {
-    const _Float16* vs = ks + MAT;
-    float s[2][16];
-    {
-      float16_t acc[2] = {};
-      auto fragment = [&](int n) {
-        const int kr = 32 * (n & 1) + (lane & 31);
-        return *reinterpret_cast<const half8_t*>(ks + kr * D + 8 * key_chunk<D>(kr, 2 * (n >> 1) + half));
-      };
-      half8_t k[AHEAD];  // reads stay AHEAD of their products
+  // S^T = K Q^T of 32 keys, `between(n)` after each of its D / 16 products; fragment reads stay AHEAD of them
+  auto scores = [&](const _Float16* ks, auto between) {
+    auto fragment = [&](int n) {
+      const int kr = lane & 31;
+      return *reinterpret_cast<const half8_t*>(ks + kr * D + 8 * key_chunk<D>(kr, 2 * n + half));
+    };
+    half8_t k[AHEAD];
+    float16_t acc = {};
 #pragma unroll
-      for (int n = 0; n < AHEAD; ++n) k[n] = fragment(n);
+    for (int n = 0; n < AHEAD; ++n) k[n] = fragment(n);
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) {
-        __builtin_amdgcn_sched_barrier(0);
-        acc[n & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n % AHEAD], q[n >> 1], acc[n & 1], 0, 0, 0);
-        if (n + AHEAD < D / 8) k[n % AHEAD] = fragment(n + AHEAD);
-      }
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[kb][e] = acc[kb][e];
+    for (int n = 0; n < D / 16; ++n) {
+      __builtin_amdgcn_sched_barrier(0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[n % AHEAD], q[n], acc, 0, 0, 0);
+      if (n + AHEAD < D / 16) k[n % AHEAD] = fragment(n + AHEAD);
+      between(n);
     }
-    // lane: row lane % 32, keys 32 kb + 8 (e / 4) + 4 half + e % 4
-    const int first = t * kWideKeys;
-    const bool hidden = first + kWideKeys > full;
-    if (hidden || ~seen) {
+    __builtin_amdgcn_sched_barrier(0);
+    return acc;
+  };
+  // the scores of keys [first, first + 32); edge: some may not be seen by some row
+  auto take = [&](const float16_t& acc, int first, bool edge, uint32_t seen) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = acc[e];
+    if (edge) {
       // this lane's keys counted from 4 half: what it sees of them as bits
       const int sees = limit - first - 4 * half;
-      const uint64_t left = seen >> (4 * half);
-      const uint64_t bits = sees <= 0 ? 0 : sees >= 64 ? left : left & ((1ull << sees) - 1);
-      const uint32_t word[2] = {(uint32_t)bits, (uint32_t)(bits >> 32)};
+      const uint32_t left = seen >> (4 * half);
+      const uint32_t bits = sees <= 0 ? 0 : sees >= 32 ? left : left & ((1u << sees) - 1);
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (!(word[kb] & (1u << (8 * (e / 4) + e % 4)))) s[kb][e] = -kInfinity;
+      for (int e = 0; e < 16; ++e)
+        if (!(bits & (1u << (8 * (e / 4) + e % 4)))) s[e] = -kInfinity;
     }
-    float top = s[0][0];
-#pragma unroll
-    for (int e = 1; e < 32; ++e) top = fmaxf(top, s[e / 16][e % 16]);
-    top = fmaxf(top, __shfl_xor(top, 32));
+  };
+  auto rescale = [&]() {
     float alpha;
-    if (weights<32>(s[0], top, m, l, alpha, c)) {
+    if (raise(max32(top), m, alpha, c)) {
+      l *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] *= alpha;
     }
-    half8_t p[2][2];
+  };
+  // weights of the scores in s, with the scores of the next 32 keys (of ks) on the matrix cores meanwhile if
+  // NEXT; then O^T += V^T P^T for the 32 rows of values at vs, and the new scores' maximum meanwhile
+  auto advance = [&](auto next, const _Float16* ks, const _Float16* vs, int first, bool edge, uint32_t seen) {
+    constexpr bool NEXT = decltype(next)::value;
+    const float mc = m == -kInfinity ? 0.0f : m * c;
+    uint32_t p[8];
+    auto weigh = [&](int i) {  // two scores to weights; the sum is of the weights as the product takes them
+      const float2_t w = {__builtin_amdgcn_exp2f(s[2 * i] * c - mc), __builtin_amdgcn_exp2f(s[2 * i + 1] * c - mc)};
+      p[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(w, half2_t));
+      l = dot2(p[i], 0x3C003C00u, l);
+    };
+    if constexpr (NEXT) {
+      const float16_t acc = scores(ks, [&](int n) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      p[kb][0] = pack8(&s[kb][0]);
-      p[kb][1] = pack8(&s[kb][8]);
+        for (int i = 0; i < 128 / D; ++i) weigh(128 / D * n + i);
+      });
+      take(acc, first, edge, seen);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) weigh(i);
     }
-    __builtin_amdgcn_sched_barrier(0);  // keeps the second product's reads behind the scores: registers
     // a transposed read gives lane d of 16 four keys' values: rows of four, 16 dimensions of each
     auto values = [&](int n) {
-      const int r0 = 16 * (n / DB) + 4 * half + ((lane & 15) >> 2);
-      const int chunk = value_chunk<D>(r0, 4 * (n % DB) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1));
-      const _Float16* at = vs + r0 * D + 8 * chunk + 4 * (lane & 1);
+      const int vr = 16 * (n / DB) + 4 * half + ((lane & 15) >> 2);
+      const int chunk = value_chunk<D>(vr, 4 * (n % DB) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1));
+      const _Float16* at = vs + vr * D + 8 * chunk + 4 * (lane & 1);
       return join(read_transposed(at), read_transposed(at + 8 * D));
     };
     half8_t v[AHEAD];
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n) v[n] = values(n);
+    top = -kInfinity;
 #pragma unroll
-    for (int n = 0; n < 4 * DB; ++n) {
+    for (int n = 0; n < 2 * DB; ++n) {
       __builtin_amdgcn_sched_barrier(0);
-      o[n % DB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[n % AHEAD], p[n / DB / 2][n / DB % 2], o[n % DB], 0, 0, 0);
-      if (n + AHEAD < 4 * DB) v[n % AHEAD] = values(n + AHEAD);
+      const int w = 4 * (n / DB);
+      const half8_t weight = __builtin_bit_cast(half8_t, make_uint4(p[w], p[w + 1], p[w + 2], p[w + 3]));
+      o[n % DB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[n % AHEAD], weight, o[n % DB], 0, 0, 0);
+      if (n + AHEAD < 2 * DB) v[n % AHEAD] = values(n + AHEAD);
+      if constexpr (NEXT) {
+#pragma unroll
+        for (int e = 8 / DB * n; e < 8 / DB * (n + 1); ++e) top = fmaxf(top, s[e]);
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  // tiles from `clear` on hold keys that some row of the workgroup does not see
-  const int clear = r.prefix ? 0x7FFFFFFF : r.behind + seg.tile * x.per + 1;
+  // Tiles up to `safe` are seen whole by every row of the workgroup.
+  const int safe = r.prefix ? r.keys : r.behind + seg.tile * x.per + 1;
   bool odd = false;
-  keys.begin(seg.t0 * kWideKeys);
-  __syncthreads();  // the tiles' place is free
-  uint64_t seen = stage(seg.t0, lds);
-  for (int t = seg.t0; t < seg.t1; ++t) {
-    _Float16* const here = lds + ((t - seg.t0) & 1) * 2 * MAT;
-    // this wave's rows have landed; after the barrier everyone's, and the other stage is free
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if ((t + 1) * kWideKeys > clear) {
+  // K of two tiles, V of two
+  auto place = [&](int t) { return lds + ((t - seg.t0) & 1) * MAT; };
+  // A tile's way: its rows are found and its K loaded two tiles ahead, its V one.  `edge`: not all of it is seen by
+  // all rows; `seen`: its keys that are there.
+  Tile rows, rows1;
+  bool edge, edge1 = false;
+  uint64_t seen, seen1 = 0;
+  auto find = [&](int t, Tile& to, bool& to_edge, uint64_t& to_seen) {
+    const int from = t * kWideKeys;
+    to.find(keys, from, r0);
+    to_edge = from + kWideKeys > safe || !to.fast;
+    to_seen = to.fast ? ~0ull : (uint64_t)__ballot(keys.page(from + lane) >= 0);
+    to.load(keys, from, r0, keys.k, k_lane, place(t));
+  };
+  auto load_v = [&](int t, const Tile& of) { of.load(keys, t * kWideKeys, r0, keys.v, v_lane, place(t) + 2 * MAT); };
+  auto step = [&](int t, auto more1, auto more2) {  // of tiles t + 1 and t + 2
+    constexpr bool MORE1 = decltype(more1)::value, MORE2 = decltype(more2)::value;
+    const _Float16 *ks = place(t), *vs = ks + 2 * MAT;
+    // V(t) has landed (K(t + 1) may be on its way), this wave's rows and after the barrier everyone's;
+    // nobody reads V(t - 1) any more
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MORE1 ? N : 0) : "memory");
+    if ((t + 1) * kWideKeys > safe && !r.prefix) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) odd |= clear_odd(here + MAT + (wr * RPW + n * RPI) * D + 8 * lane);
+      for (int n = 0; n < N; ++n) odd |= clear_odd(place(t) + 2 * MAT + (r0 + n * RPI) * D + 8 * lane);
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const uint64_t now = seen;
-    if (t + 1 < seg.t1) seen = stage(t + 1, lds + ((t + 1 - seg.t0) & 1) * 2 * MAT);
-    if (wave_live) compute(t, now, here);
+    if constexpr (MORE1) load_v(t + 1, rows1);
+    if (wave_live) {
+      advance(std::true_type{}, ks + 32 * D, vs, t * kWideKeys + 32, edge, (uint32_t)(seen >> 32));
+      rescale();
+    }
+    if constexpr (MORE1) {
+      // the same of K(t + 1), V(t + 1) and K(t)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+    }
+    edge = edge1;
+    seen = seen1;
+    if constexpr (MORE2) {
+      keys.reach((t + 2) * kWideKeys);
+      find(t + 2, rows1, edge1, seen1);
+    }
+    if (wave_live) {
+      advance(more1, place(t + 1), vs + 32 * D, (t + 1) * kWideKeys, edge, (uint32_t)seen);
+      if constexpr (MORE1) rescale();
+    }
+  };
+
+  keys.begin(seg.t0 * kWideKeys);
+  settle(q);
+  __syncthreads();  // the tiles' places are free
+  find(seg.t0, rows, edge, seen);
+  load_v(seg.t0, rows);
+  if (seg.t0 + 1 < seg.t1) {
+    keys.reach((seg.t0 + 1) * kWideKeys);
+    find(seg.t0 + 1, rows1, edge1, seen1);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * N) : "memory");
+  } else {
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
   }
+  if (wave_live) {
+    take(scores(place(seg.t0), [](int) {}), seg.t0 * kWideKeys, edge, (uint32_t)seen);
+    top = s[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+    rescale();
+  }
+  int t = seg.t0;
+  for (; t + 2 < seg.t1; ++t) step(t, std::true_type{}, std::true_type{});
+  if (t + 1 < seg.t1) {
+    step(t, std::true_type{}, std::false_type{});
+    ++t;
+  }
+  step(t, std::false_type{}, std::false_type{});
   l += __shfl_xor(l, 32);
   if (__syncthreads_or(odd)) {
-    for (int key = max(seg.t0, max(clear, 0) / kWideKeys) * kWideKeys; key < min(seg.t1 * kWideKeys, bound); ++key) {
+    for (int key = max(seg.t0, max(safe, 0) / kWideKeys) * kWideKeys; key < min(seg.t1 * kWideKeys, bound); ++key) {
       const int page = keys.entry(key >> x.page_shift);
       if (page < 0 || key >= limit) continue;
       const _Float16* v = keys.v + keys.at(page, key) + 4 * half;
@@ -336,9 +497,9 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
 // One segment of a narrow item by one wave: up to 16 rows against key tiles [t0, t1).
 template <int D>
 __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Extents& x, const Request& r, const Segment& seg,
-                                               const int32_t* pages, float* slot, bool whole, _Float16* lds) {
+                                               const int32_t* pages, float* slot, bool whole, _Float16* lds, int32_t* ring) {
   constexpr int CH = D / 8, RPI = 512 / D, N = kNarrowKeys / RPI, MAT = kNarrowKeys * D, DB = D / 16;
-  const int lane = threadIdx.x & 63, quad = lane >> 4, row = lane & 15;
+  const int lane = here() & 63, quad = lane >> 4, row = lane & 15;
   const int i = row / x.share, j = row - i * x.share;
   const bool live = i < r.count;
   const int bound = r.keys;
@@ -352,44 +513,56 @@ __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Ext
 #pragma unroll
     for (int kk = 0; kk < D / 32; ++kk) q[kk] = *reinterpret_cast<const half8_t*>(src + 32 * kk + 8 * quad);
   }
-  Keys<D> keys(a, seg.head, pages, bound);
-  auto stage = [&](int t, const _Float16* matrix, bool values, _Float16* dst) {
+  Keys<D> keys(a, seg.head, pages, bound, ring, lane);
+  using Tile = Rows<D, kNarrowKeys, N>;
+  uint32_t k_lane[N], v_lane[N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int kr = n * RPI + lane / CH, key = t * kNarrowKeys + kr, p = keys.page(key);
-      const int chunk = values ? value_chunk<D>(kr, lane % CH) : key_chunk<D>(kr, lane % CH);
-      dma16(p < 0 ? (const void*)zeros : matrix + keys.at(p, key) + 8 * chunk, dst + n * RPI * D);
-    }
-  };
+  for (int n = 0; n < N; ++n) {
+    const int kr = n * RPI + lane / CH;
+    k_lane[n] = 2 * ((lane / CH) * D + 8 * key_chunk<D>(kr, lane % CH));
+    v_lane[n] = 2 * ((lane / CH) * D + 8 * value_chunk<D>(kr, lane % CH));
+  }
   float4_t o[DB] = {};
   float m = -kInfinity, l = 0.0f;
   bool odd = false;
+  Tile rows;
+  uint32_t seen, seen1 = 0;
+  auto find = [&](int t, uint32_t& to_seen) {
+    rows.find(keys, t * kNarrowKeys, 0);
+    to_seen = rows.fast ? ~0u : (uint32_t)__ballot(keys.page(t * kNarrowKeys + (lane & 31)) >= 0);
+    rows.load(keys, t * kNarrowKeys, 0, keys.k, k_lane, lds);
+  };
   keys.begin(seg.t0 * kNarrowKeys);
-  stage(seg.t0, keys.k, false, lds);
-  stage(seg.t0, keys.v, true, lds + MAT);
+  settle(q);
+  find(seg.t0, seen);
+  rows.load(keys, seg.t0 * kNarrowKeys, 0, keys.v, v_lane, lds + MAT);
   for (int t = seg.t0; t < seg.t1; ++t) {
     const bool more = t + 1 < seg.t1;
-    const uint32_t seen = (uint32_t)__ballot(keys.page(t * kNarrowKeys + (lane & 31)) >= 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (!r.prefix && (t + 1) * kNarrowKeys > full) {  // keys that some row does not see
-#pragma unroll
-      for (int n = 0; n < N; ++n) odd |= clear_odd(lds + MAT + n * RPI * D + 8 * lane);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");  // K(t) has landed, V(t) is on its way
     float s[8];
+    {
+      half8_t k[2][D / 32];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      float4_t acc = {};
+      for (int kk = 0; kk < D / 32; ++kk)
 #pragma unroll
-      for (int kk = 0; kk < D / 32; ++kk) {
-        const int kr = 16 * kb + row;
-        const half8_t k = *reinterpret_cast<const half8_t*>(lds + kr * D + 8 * key_chunk<D>(kr, 4 * kk + quad));
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[kk], acc, 0, 0, 0);
-      }
+        for (int kb = 0; kb < 2; ++kb) {
+          const int kr = 16 * kb + row;
+          k[kb][kk] = *reinterpret_cast<const half8_t*>(lds + kr * D + 8 * key_chunk<D>(kr, 4 * kk + quad));
+        }
+      float4_t acc[2] = {};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[4 * kb + e] = acc[e];
+      for (int kk = 0; kk < D / 32; ++kk)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) acc[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[kb][kk], q[kk], acc[kb], 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = acc[e / 4][e % 4];
     }
-    // lane: row lane % 16, keys 16 kb + 4 quad + e
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K(t) has been read
+    if (more) {
+      keys.reach((t + 1) * kNarrowKeys);
+      find(t + 1, seen1);
+    }
+    // lane: row lane % 16, keys 16 (e / 4) + 4 quad + e % 4
     const int first = t * kNarrowKeys;
     if (first + kNarrowKeys > full || ~seen) {
       const int sees = limit - first - 4 * quad;
@@ -402,28 +575,42 @@ __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Ext
     float top = s[0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e]);
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
+    top = max32(max16(top));
     float alpha;
-    if (weights<8>(s, top, m, l, alpha, c)) {
+    if (raise(top, m, alpha, c)) {
+      l *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] *= alpha;
     }
-    const half8_t p = pack8(s);
-    auto values = [&](int db) {
-      const int r0 = 4 * quad + (row >> 2), chunk = value_chunk<D>(r0, 2 * db + ((lane & 3) >> 1));
-      const _Float16* at = lds + MAT + r0 * D + 8 * chunk + 4 * (lane & 1);
-      return join(read_transposed(at), read_transposed(at + 16 * D));
-    };
+    const float mc = m == -kInfinity ? 0.0f : m * c;
+    uint32_t p[4];
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
-      o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values(db), p, o[db], 0, 0, 0);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile has been read
-    if (more) {
-      keys.reach((t + 1) * kNarrowKeys);
-      stage(t + 1, keys.k, false, lds);
-      stage(t + 1, keys.v, true, lds + MAT);
+    for (int i = 0; i < 4; ++i) {
+      const float2_t w = {__builtin_amdgcn_exp2f(s[2 * i] * c - mc), __builtin_amdgcn_exp2f(s[2 * i + 1] * c - mc)};
+      p[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(w, half2_t));
+      l = dot2(p[i], 0x3C003C00u, l);
     }
+    const half8_t weight = __builtin_bit_cast(half8_t, make_uint4(p[0], p[1], p[2], p[3]));
+    // V(t) has landed, K(t + 1) is on its way
+    if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (!r.prefix && first + kNarrowKeys > full) {  // keys that some row does not see
+#pragma unroll
+      for (int n = 0; n < N; ++n) odd |= clear_odd(lds + MAT + n * RPI * D + 8 * lane);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    half8_t v[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      const int vr = 4 * quad + (row >> 2), chunk = value_chunk<D>(vr, 2 * db + ((lane & 3) >> 1));
+      const _Float16* at = lds + MAT + vr * D + 8 * chunk + 4 * (lane & 1);
+      v[db] = join(read_transposed(at), read_transposed(at + 16 * D));
+    }
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[db], weight, o[db], 0, 0, 0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V(t) has been read
+    if (more) rows.load(keys, (t + 1) * kNarrowKeys, 0, keys.v, v_lane, lds + MAT);
+    seen = seen1;
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
@@ -460,42 +647,51 @@ __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Ext
   }
 }
 
+// A token's rows in the slots of one list, as the joining kernel reads them: half a record.
+struct TokenPart {
+  TokenSlots at;
+  int quota, narrow;
+};
+static_assert(sizeof(TokenPart) == 2 * kRecord, "a record is two parts");
+
 // Every workgroup plans the whole call itself (a scan over the requests' key tiles), takes an equal
 // share of the wide tiles and each of its waves an equal share of the narrow ones.
 template <int D>
 __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
   __shared__ __attribute__((aligned(16))) _Float16 tiles[kWaves * 8192];
-  __shared__ int32_t starts[2][kAttentionMaxRequests + 2];
-  __shared__ int32_t sums[2][kWaves];
+  __shared__ __attribute__((aligned(16))) int32_t rings[kWaves][128];
+  __shared__ int32_t starts[3][kAttentionMaxRequests + 2];
+  __shared__ int32_t sums[3][kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  const Extents x = extents_of(a);
+  Extents x = extents_of(a);
   const int lists = a.requests + 1;
-  int done[2] = {0, 0};  // tiles of the wide and the narrow list
+  int done[3] = {0, 0, 0};  // tiles of the wide and the narrow list, items of the wide one
   for (int base = 0; base < lists; base += kThreads) {
     const int b = base + tid;
-    int mine[2] = {0, 0};
+    int mine[3] = {0, 0, 0};
     if (b < lists) {
       const Request r = request_of(a, x, b);
-      const int n = a.kv * (int)head_tiles(x, r);
-      mine[0] = r.narrow ? 0 : n;
-      mine[1] = r.narrow ? n : 0;
+      const int span = a.kv * head_span(x, r);
+      mine[0] = r.narrow ? 0 : span;
+      mine[1] = r.narrow ? span : 0;
+      mine[2] = a.kv * head_items(x, r);
     }
-    int scan[2] = {mine[0], mine[1]};
+    int scan[3] = {mine[0], mine[1], mine[2]};
 #pragma unroll
     for (int step = 1; step < 64; step <<= 1)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < 3; ++k) {
         const int below = __shfl_up(scan[k], step);
         if (lane >= step) scan[k] += below;
       }
     __syncthreads();
     if (lane == 63) {
-      sums[0][wave] = scan[0];
-      sums[1][wave] = scan[1];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) sums[k][wave] = scan[k];
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < 3; ++k) {
       int before = done[k];
       for (int w = 0; w < kWaves; ++w) {
         if (w < wave) before += sums[k][w];
@@ -504,150 +700,177 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
       if (b < lists) starts[k][b] = before + scan[k] - mine[k];
     }
   }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) done[k] = uniform(done[k]);
+  x.cost = item_cost(done[0]);
+  if (x.cost)  // each thread its own entries
+    for (int b = tid; b < lists; b += kThreads) starts[0][b] += x.cost * starts[2][b];
+  done[0] += x.cost * done[2];
   if (tid < 2) starts[tid][lists] = tid ? done[1] : done[0];
   __syncthreads();
   const int quota[2] = {(done[0] + kGroups - 1) / kGroups, (done[1] + kStreams - 1) / kStreams};
-  if (blockIdx.x == 0) {  // for the kernel that joins the segments
-    int32_t* plan = static_cast<int32_t*>(a.workspace);
-    if (tid < 2) plan[tid] = tid ? quota[1] : quota[0];
-    for (int b = tid; b <= lists; b += kThreads) {
-      plan[2 + b] = starts[0][b];
-      plan[3 + lists + b] = starts[1][b];
-    }
-  }
   const bool alone = prefix_request(x, a.tokens, *a.prefix_length).keys == 0;
-  float* const slots = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + plan_bytes(a.requests));
+  float* const slots = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + record_bytes(a.tokens));
 
-  const int wide_end = min((int)(blockIdx.x + 1) * quota[0], done[0]);
-  for (int t = (int)blockIdx.x * quota[0]; t < wide_end;) {
-    const int b = uniform(find(starts[0], lists, t));
-    const Request r = request_of(a, x, b);
-    Segment seg = segment_at(x, r, b, (starts[0][b + 1] - starts[0][b]) / a.kv, t - starts[0][b],
-                             wide_end - t);
-    seg.head = uniform(seg.head);
-    seg.tile = uniform(seg.tile);
-    seg.t0 = uniform(seg.t0);
-    seg.t1 = uniform(seg.t1);
-    wide_segment<D>(a, x, r, seg, r.prefix ? a.prefix_pages : a.table + (size_t)b * a.columns,
-                    slots + slot_floats(kWideRows, D) * (size_t)(seg.item + blockIdx.x), alone && !r.prefix && seg.all,
-                    tiles);
-    t += seg.t1 - seg.t0;
+  const auto requests = [&](int b) { return request_of(a, x, b); };
+  auto list_of = [&](const Request& r, int b) { return r.prefix ? a.prefix_pages : a.table + (size_t)b * a.columns; };
+  // what is the same in the whole wave, in scalar registers
+  auto settle = [&](Walk<decltype(requests)>& walk) {
+    walk.left = uniform(walk.left);
+    walk.b = uniform(walk.b);
+    walk.head = uniform(walk.head);
+    walk.tile = uniform(walk.tile);
+    walk.at = uniform(walk.at);
+    walk.r.first = uniform(walk.r.first);
+    walk.r.count = uniform(walk.r.count);
+    walk.r.keys = uniform(walk.r.keys);
+    walk.r.behind = uniform(walk.r.behind);
+    walk.r.prefix = uniform(walk.r.prefix);
+    walk.r.narrow = uniform(walk.r.narrow);
+  };
+  auto wide_list = [&]() {
+    // Workgroups go round the eight XCDs in turn: neighbouring ranges, which read the same keys, are given to
+    // one XCD, whose L2 then serves most of them.
+    const int ranges = quota[0] ? (done[0] + quota[0] - 1) / quota[0] : 0, share = (ranges + 7) / 8;
+    const int range = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= share || range >= ranges) return;
+    Walk<decltype(requests)> walk(x, starts[0], requests, range * quota[0], min((range + 1) * quota[0], done[0]));
+    Segment seg;
+    for (settle(walk); walk.next(seg); walk.advance(), settle(walk)) {
+      wide_segment<D>(a, x, walk.r, seg, list_of(walk.r, walk.b),
+                      slots + slot_floats(kWideRows, D) * (size_t)(seg.item + range), alone && !walk.r.prefix && seg.all,
+                      tiles, rings[wave]);
+    }
+  };
+  auto narrow_list = [&]() {
+    float* const base = slots + slot_floats(kWideRows, D) * (size_t)wide_slots(x);
+    const int stream = wave * kGroups + blockIdx.x;  // neighbours in the list run on different CUs
+    const int from = stream * quota[1], to = min(from + quota[1], done[1]);
+    if (from >= to) return;
+    Walk<decltype(requests)> walk(x, starts[1], requests, from, to);
+    Segment seg;
+    for (settle(walk); walk.next(seg); walk.advance(), settle(walk)) {
+      narrow_segment<D>(a, x, walk.r, seg, list_of(walk.r, walk.b),
+                        base + slot_floats(kNarrowRows, D) * (size_t)(seg.item + stream), alone && !walk.r.prefix && seg.all,
+                        tiles + wave * 2 * kNarrowKeys * D, rings[wave]);
+    }
+  };
+  // The wide list is bound by arithmetic, the narrow one by memory: the second half of the workgroups, which
+  // share CUs with the first, takes them in the other order.
+  for (int turn = 0; turn < 2; ++turn) {
+    if ((blockIdx.x >= kGroups / 2) == (turn == 1)) wide_list();
+    else narrow_list();
+    __syncthreads();
   }
-  __syncthreads();
-  float* const narrow_base = slots + slot_floats(kWideRows, D) * (size_t)wide_slots(x);
-  const int stream = wave * kGroups + blockIdx.x;  // neighbours in the list run on different CUs
-  const int narrow_end = min((stream + 1) * quota[1], done[1]);
-  for (int t = stream * quota[1]; t < narrow_end;) {
-    const int b = uniform(find(starts[1], lists, t));
+  // Where the joining kernel finds each token's slots, worked out by the last workgroups, which have the least
+  // other work in small calls.
+  for (int t = (kGroups - 1 - (int)blockIdx.x) * kThreads + tid; t < a.tokens; t += kGroups * kThreads) {
+    TokenPart* record = static_cast<TokenPart*>(a.workspace) + 2 * (size_t)t;
+    const Request all = request_of(a, x, a.requests);
+    const int b = find(a.offsets, a.requests, t);
     const Request r = request_of(a, x, b);
-    Segment seg = segment_at(x, r, b, (starts[1][b + 1] - starts[1][b]) / a.kv, t - starts[1][b],
-                             narrow_end - t);
-    seg.head = uniform(seg.head);
-    seg.t0 = uniform(seg.t0);
-    seg.t1 = uniform(seg.t1);
-    narrow_segment<D>(a, x, r, seg, r.prefix ? a.prefix_pages : a.table + (size_t)b * a.columns,
-                      narrow_base + slot_floats(kNarrowRows, D) * (size_t)(seg.item + stream),
-                      alone && !r.prefix && seg.all, tiles + wave * 2 * kNarrowKeys * D);
-    t += seg.t1 - seg.t0;
+    TokenPart shared{}, mine{};
+    if (t < all.count && t >= r.first && t < r.first + r.count) {
+      shared = TokenPart{token_slots(x, all, a.requests, starts[all.narrow][a.requests], t), all.narrow ? quota[1] : quota[0], all.narrow};
+      mine = TokenPart{token_slots(x, r, b, starts[r.narrow][b], t), r.narrow ? quota[1] : quota[0], r.narrow};
+    }
+    record[0] = shared;
+    record[1] = mine;
   }
 }
 
-// Joins the segments of a token's query heads: out = sum_p w_p O_p / sum_p w_p l_p, w_p = exp(m_p - max m).
-// A workgroup takes one or all key heads of a token (HEADS; what the token's place in the plan costs is then
-// shared), a thread four dimensions of a query head; threads beyond those of a key head share its segments.
+// Joins the segments of a row (a token's query head): out = sum_p w_p O_p / sum_p w_p l_p, w_p = exp(m_p - max m).
+// D / 4 lanes, each with four dimensions, take a row, or (split > 1) as many sets of lanes share its segments and
+// are added up through LDS.  A segment's maximum and sum are in one lane each, so that a lane computes one
+// weight for all dimensions and the outputs' loads wait for nothing but the record.
 template <int D, int THREADS>
-__global__ __launch_bounds__(THREADS) void join_segments(const AttentionArgs a, int heads) {
-  constexpr int VECS = D / 4, BATCH = 4;
-  const int groups = a.kv / heads;
-  const int token = blockIdx.x / groups, first_head = (blockIdx.x - token * groups) * heads;
-  const int tid = threadIdx.x, lane = tid & 63;
+__global__ __launch_bounds__(THREADS) void join_segments(const AttentionArgs a, int split) {
+  constexpr int LANES = D / 4, SETS = THREADS / LANES, BATCH = 8;
+  const int tid = threadIdx.x, lane = tid % LANES, set = tid / LANES, part = set % split;
+  const int per = SETS / split, rows_all = a.tokens * a.heads, row = blockIdx.x * per + set / split;
   const Extents x = extents_of(a);
   const float c = a.scale * 1.44269504088896340736f;
-  const Request all = request_of(a, x, a.requests);
-  const int32_t* plan = static_cast<const int32_t*>(a.workspace);
-  const float* const slots = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.workspace) + plan_bytes(a.requests));
-  const float* const narrow_base = slots + slot_floats(kWideRows, D) * (size_t)wide_slots(x);
-
-  struct Part {  // the token's rows in the slots of one list
-    TokenSlots at;
-    const float* base;
-    int rows, quota;
+  const int here = min(row, rows_all - 1), token = here / a.heads, head = here - token * a.heads;
+  const int kv_head = head / x.share, j = head - kv_head * x.share;
+  TokenPart parts[2];  // in the prefix's list and in its request's own
+  __builtin_memcpy(parts, static_cast<const TokenPart*>(a.workspace) + 2 * (size_t)token, sizeof(parts));
+  const float* const slots = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.workspace) + record_bytes(a.tokens));
+  const float* from[2];  // the row's maximum in its first slot
+  size_t stride[2];
+  int count[2], sum_at[2], out_at[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const Slots s = parts[k].at.in(kv_head, parts[k].quota);
+    const int rows = parts[k].narrow ? kNarrowRows : kWideRows, at = parts[k].at.row + j;
+    count[k] = s.count;
+    stride[k] = slot_floats(rows, D);
+    from[k] = slots + (parts[k].narrow ? slot_floats(kWideRows, D) * (size_t)wide_slots(x) : 0) + stride[k] * (size_t)s.first + at;
+    sum_at[k] = rows;
+    out_at[k] = 2 * rows + at * (D - 1) + 4 * lane;
+  }
+  const int all = count[0] + count[1];
+  auto slot = [&](int p, bool k) { return from[k] + stride[k] * (size_t)(k ? p - count[0] : p); };
+  // over the lanes of a set
+  auto highest = [&](float v) {
+#pragma unroll
+    for (int step = LANES / 2; step > 0; step >>= 1) v = fmaxf(v, __shfl_xor(v, step));
+    return v;
   };
-  auto part = [&](const Request& r, int b) {
-    return Part{token_slots(x, r, b, plan[2 + (r.narrow ? a.requests + 2 : 0) + b], token), r.narrow ? narrow_base : slots,
-                r.narrow ? kNarrowRows : kWideRows, plan[r.narrow ? 1 : 0]};
-  };
-  Part shared{}, mine{};
-  if (token < all.count) {
-    int b = 0;  // the token's request: offsets[b] <= token
-    for (int i = 1; i < a.requests; i += 64)
-      b += __popcll(__ballot(i + lane < a.requests && a.offsets[min(i + lane, a.requests)] <= token));
-    const Request r = request_of(a, x, b);
-    if (token >= r.first && token < r.first + r.count) {
-      shared = part(all, a.requests);
-      mine = part(r, b);
+  auto weight = [&](float v, float top) { return v == -kInfinity ? 0.0f : __builtin_amdgcn_exp2f((v - top) * c); };
+  // this set's segments: part, part + split, ..
+  float m = -kInfinity, l = 0.0f;
+  float4_t o = {};
+  for (int p0 = part; p0 < all; p0 += split * LANES) {
+    const int n = min(LANES, (all - p0 + split - 1) / split);
+    float4_t op[BATCH];
+    auto load = [&](int i0) {
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int p = p0 + min(i0 + i, n - 1) * split;
+        op[i] = *reinterpret_cast<const float4_t*>(slot(p, p >= count[0]) + out_at[p >= count[0]]);
+      }
+    };
+    const int mine = p0 + min(lane, n - 1) * split;
+    const float* at = slot(mine, mine >= count[0]);
+    float mp = at[0], lp = at[sum_at[mine >= count[0]]];
+    load(0);
+    if (lane >= n) mp = -kInfinity;
+    const float top = highest(fmaxf(m, mp)), w = weight(mp, top), f = weight(m, top);
+    m = top;
+    l = l * f + (lane < n ? w * lp : 0.0f);
+    o *= f;
+    for (int i0 = 0; i0 < n; i0 += BATCH) {
+      if (i0) load(i0);
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const float wi = __shfl(w, min(i0 + i, LANES - 1), LANES);
+        if (i0 + i < n) o += op[i] * wi;
+      }
     }
   }
-  const int vecs = x.share * VECS, sets = vecs < THREADS ? THREADS / vecs : 1, set = tid / vecs;
-  __shared__ float4_t outs[THREADS];
-  __shared__ float2 stats[THREADS];
-  for (int head = first_head; head < first_head + heads; ++head) {
-    const Slots one = shared.at.in(head, shared.quota), two = mine.at.in(head, mine.quota);
-    if (two.count == 1 && all.keys == 0) continue;  // the segment wrote the output itself
-    const int count = one.count + two.count;
-    for (int v = tid - set * vecs; v < vecs; v += THREADS) {  // more than once where sets is 1
-      const int j = v / VECS, vec = v - j * VECS;
-      float m = -kInfinity, l = 0.0f;
-      float4_t o = {};
-      if (set < sets) {
-        for (int p0 = set; p0 < count; p0 += BATCH * sets) {
-          float mp[BATCH], lp[BATCH];
-          float4_t op[BATCH];
 #pragma unroll
-          for (int n = 0; n < BATCH; ++n) {
-            const int p = min(p0 + n * sets, count - 1);
-            const bool first = p < one.count;
-            const Part& from = first ? shared : mine;
-            const int rows = first ? shared.rows : mine.rows, row = (first ? shared.at.row : mine.at.row) + j;
-            const float* slot = from.base + slot_floats(rows, D) * (size_t)(first ? one.first + p : two.first + p - one.count);
-            mp[n] = slot[row];
-            lp[n] = slot[rows + row];
-            op[n] = *reinterpret_cast<const float4_t*>(slot + 2 * rows + (size_t)row * D + 4 * vec);
-          }
+  for (int step = LANES / 2; step > 0; step >>= 1) l += __shfl_xor(l, step);
+  if (split > 1) {  // split <= LANES
+    __shared__ float4_t outs[THREADS];
+    __shared__ float2 stats[SETS];
+    outs[tid] = o;
+    if (lane == 0) stats[set] = make_float2(m, l);
+    __syncthreads();
+    if (part) return;
+    const float2 other = stats[set + min(lane, split - 1)];
+    const float ms = lane < split ? other.x : -kInfinity;
+    const float w = weight(ms, highest(ms));
+    l = lane < split ? w * other.y : 0.0f;
 #pragma unroll
-          for (int n = 0; n < BATCH; ++n) {
-            if (p0 + n * sets >= count) break;
-            const float next = fmaxf(m, mp[n]);
-            const float f = m == -kInfinity ? 0.0f : exp2f((m - next) * c);
-            const float g = mp[n] == -kInfinity ? 0.0f : exp2f((mp[n] - next) * c);
-            l = l * f + lp[n] * g;
-            o = o * f + op[n] * g;
-            m = next;
-          }
-        }
-      }
-      if (sets == 1 && set) break;  // threads beyond the key head's
-      if (sets > 1) {  // one round of this loop
-        __syncthreads();
-        outs[tid] = o;
-        stats[tid] = make_float2(m, l);
-        __syncthreads();
-        if (set) continue;
-        for (int s = 1; s < sets; ++s) {
-          const float2 other = stats[tid + s * vecs];
-          const float next = fmaxf(m, other.x);
-          const float f = m == -kInfinity ? 0.0f : exp2f((m - next) * c);
-          const float g = other.x == -kInfinity ? 0.0f : exp2f((other.x - next) * c);
-          l = l * f + other.y * g;
-          o = o * f + outs[tid + s * vecs] * g;
-          m = next;
-        }
-      }
-      const float4_t w = o * (l == 0.0f ? 0.0f : 1.0f / l);
-      *reinterpret_cast<uint2*>(static_cast<_Float16*>(a.out) + ((size_t)token * a.heads + head * x.share) * D + 4 * v) =
-          make_uint2(half2_from_fp32(w[0], w[1]), half2_from_fp32(w[2], w[3]));
-    }
+    for (int step = LANES / 2; step > 0; step >>= 1) l += __shfl_xor(l, step);
+    o = float4_t{};
+    for (int s = 0; s < split; ++s) o += outs[tid + s * LANES] * __shfl(w, s, LANES);
   }
+  // rows whose only segment wrote the output itself
+  if (row >= rows_all || (count[1] == 1 && parts[0].at.tiles == 0)) return;
+  const float4_t v = o * (l == 0.0f ? 0.0f : 1.0f / l);
+  *reinterpret_cast<uint2*>(static_cast<_Float16*>(a.out) + (size_t)row * D + 4 * lane) =
+      make_uint2(half2_from_fp32(v[0], v[1]), half2_from_fp32(v[2], v[3]));
 }
 
 template <int D>
@@ -655,13 +878,15 @@ hipError_t launch_dim(const AttentionArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL((attend<D>), dim3(kGroups), dim3(kThreads), 0, stream, a);
   hipError_t status = hipGetLastError();
   if (status != hipSuccess) return status;
-  const int64_t units = (int64_t)a.tokens * a.kv;
-  if (units <= kGroups)
-    hipLaunchKernelGGL((join_segments<D, 1024>), dim3((unsigned)units), dim3(1024), 0, stream, a, 1);
-  else if (a.tokens < 4 * kGroups)
-    hipLaunchKernelGGL((join_segments<D, 256>), dim3((unsigned)units), dim3(256), 0, stream, a, 1);
-  else
-    hipLaunchKernelGGL((join_segments<D, 256>), dim3((unsigned)a.tokens), dim3(256), 0, stream, a, a.kv);
+  // few rows: more lanes for each
+  constexpr int lanes = D / 4;
+  const int rows = a.tokens * a.heads;
+  int split = 1;
+  while (split < 16 && (int64_t)rows * split < 8192) split *= 2;
+  const int threads = split * lanes > 256 ? 512 : 256, per = threads / lanes / split;
+  const dim3 grid((unsigned)(((int64_t)rows + per - 1) / per));
+  if (threads == 512) hipLaunchKernelGGL((join_segments<D, 512>), grid, dim3(512), 0, stream, a, split);
+  else hipLaunchKernelGGL((join_segments<D, 256>), grid, dim3(256), 0, stream, a, split);
   return hipGetLastError();
 }
 
@@ -669,7 +894,7 @@ hipError_t launch_dim(const AttentionArgs& a, hipStream_t stream) {
 
 size_t attention_workspace(const AttentionArgs& a) {
   const Extents x = extents_of(a);
-  return plan_bytes(a.requests) + 4 * (slot_floats(kWideRows, a.dim) * (size_t)wide_slots(x) +
+  return record_bytes(a.tokens) + 4 * (slot_floats(kWideRows, a.dim) * (size_t)wide_slots(x) +
                                        slot_floats(kNarrowRows, a.dim) * (size_t)narrow_slots(x));
 }
 

@@ -7,14 +7,16 @@
 // each workgroup, the narrow list into equal ranges, one for each wave; a range crosses items, so the
 // work is even whatever the lengths.  The part of an item in one range is a segment; it leaves its
 // rows' maxima, sums and outputs in a slot of the workspace, and a second kernel joins the slots of a row.
-// Slot = item + range: both only grow along the list, one of them with every segment.
+// Slot = item + range: both only grow along the list, one of them with every segment.  To begin a wide item
+// costs a workgroup as much as kItemCost tiles, so in long lists each has that many empty positions before its
+// first tile (in short ones a range of one more tile would cost more than it evens out).
 #pragma once
 
 #include <stddef.h>
 #include <stdint.h>
 
 #ifdef __HIP__
-#define PAGED_CODE __host__ __device__ inline
+#define PAGED_CODE __host__ __device__ __forceinline__
 #else
 #define PAGED_CODE inline
 #endif
@@ -25,6 +27,7 @@ constexpr int kWaves = 4;                   // of a workgroup
 constexpr int kGroups = 512;                // workgroups: two per CU
 constexpr int kStreams = kGroups * kWaves;  // waves of the launch
 constexpr int kWideRows = 128, kWideKeys = 64, kNarrowRows = 16, kNarrowKeys = 32;
+constexpr int kItemCost = 3, kLongRange = 24;  // tiles of a range from which items have a cost
 
 PAGED_CODE int least(int a, int b) { return a < b ? a : b; }
 PAGED_CODE int most(int a, int b) { return a > b ? a : b; }
@@ -33,13 +36,16 @@ PAGED_CODE int most(int a, int b) { return a > b ? a : b; }
 struct Extents {
   int tokens, requests, kv, share, page_shift, columns, prefix_columns;  // share: query heads of a key head
   int per;                                                               // tokens of a wide row tile
+  int cost;                                                              // positions before an item's first tile
 };
 PAGED_CODE Extents extents(int tokens, int requests, int heads, int kv, int page_shift, int columns, int prefix_columns) {
   const int share = heads / kv;
-  return Extents{tokens, requests, kv, share, page_shift, columns, prefix_columns, kWideRows / share};
+  return Extents{tokens, requests, kv, share, page_shift, columns, prefix_columns, kWideRows / share, 0};
 }
 
-PAGED_CODE size_t plan_bytes(int requests) { return ((size_t)(2 + 2 * (requests + 2)) * 4 + 255) / 256 * 256; }
+// Workspace: a record of each token for the joining kernel, then wide and narrow slots.
+constexpr int kRecord = 16;  // 32-bit words
+PAGED_CODE size_t record_bytes(int tokens) { return ((size_t)tokens * 4 * kRecord + 255) / 256 * 256; }
 PAGED_CODE size_t slot_floats(int rows, int dim) { return (size_t)rows * (dim + 2); }
 PAGED_CODE int64_t wide_slots(const Extents& e) {
   return (int64_t)e.kv * (e.tokens / e.per + e.requests + (e.tokens + e.per - 1) / e.per) + kGroups;
@@ -115,14 +121,26 @@ PAGED_CODE unsigned wide_tiles(const Extents& e, const Request& r, int tiles) {
 // narrow requests' one each, by the key tiles of the longest list.  The call is refused from 2^31 on.
 PAGED_CODE int64_t most_tiles(const Extents& e) {
   const int64_t keys = (int64_t)most(e.columns, e.prefix_columns) << e.page_shift;
-  return e.kv * (e.tokens / e.per * 2 + e.requests + 3ll) * ((keys + e.tokens) / kNarrowKeys + 2) + 2 * kStreams;
+  return e.kv * (e.tokens / e.per * 2 + e.requests + 3ll) * ((keys + e.tokens) / kNarrowKeys + 2 + kItemCost) + 2 * kStreams;
 }
 
-// key tiles of one key head
-PAGED_CODE unsigned head_tiles(const Extents& e, const Request& r) {
+// Positions of one key head in its list: key tiles, and a wide item's cost.
+PAGED_CODE int head_span(const Extents& e, const Request& r) {
   if (!r.count || !r.keys) return 0;
   if (r.narrow) return (r.keys + kNarrowKeys - 1) / kNarrowKeys;
-  return wide_tiles(e, r, row_tiles(e, r));
+  return (int)wide_tiles(e, r, row_tiles(e, r)) + e.cost * row_tiles(e, r);
+}
+// Items of one key head in the wide list.
+PAGED_CODE int head_items(const Extents& e, const Request& r) { return r.count && r.keys && !r.narrow ? row_tiles(e, r) : 0; }
+PAGED_CODE int item_cost(int tiles) { return tiles >= kLongRange * kGroups ? kItemCost : 0; }  // by the wide list's tiles
+// Where row tile `tile` of a wide request begins within its key head, and the key tiles of a row tile.
+PAGED_CODE int wide_begin(const Extents& e, const Request& r, int tile) {
+  return (int)wide_tiles(e, r, tile) + e.cost * tile;
+}
+PAGED_CODE int item_tiles(const Extents& e, const Request& r, int tile) {
+  if (r.narrow) return (r.keys + kNarrowKeys - 1) / kNarrowKeys;
+  const int keys = r.prefix ? r.keys : most(r.behind, 0) + least(r.count, (tile + 1) * e.per);
+  return (keys + kWideKeys - 1) / kWideKeys;
 }
 
 // Items of request b (b = requests: the prefix) grow along the list and stay within the slots.
@@ -141,61 +159,93 @@ PAGED_CODE int find(const int32_t* start, int count, int t) {
   return lo;
 }
 
-// The segment at tile `at` of a request's list, in a range that takes `left` more tiles.
+// A range's way through its list: `requests(b)` gives request b, `start` the first position of each.
 struct Segment {
   int head, tile, t0, t1;  // key head, row tile, key tiles
   int item;
   bool all;                // the item's only segment
 };
-PAGED_CODE Segment segment_at(const Extents& e, const Request& r, int b, int per_head, int at, int left) {
-  Segment s;
-  s.head = at / per_head;
-  const int rest = at - s.head * per_head;
-  int tiles = per_head, begin = 0;
-  s.tile = 0;
-  if (!r.narrow) {
-    int lo = 0, hi = row_tiles(e, r);  // the last row tile that begins at or before rest
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if ((int)wide_tiles(e, r, mid) <= rest) lo = mid; else hi = mid;
-    }
-    s.tile = lo;
-    begin = (int)wide_tiles(e, r, lo);
-    tiles = (int)wide_tiles(e, r, lo + 1) - begin;
-  }
-  s.t0 = rest - begin;
-  s.t1 = least(tiles, s.t0 + left);
-  s.item = r.narrow ? narrow_item(e, b, s.head) : wide_item(e, r, b, s.head, s.tile);
-  s.all = s.t0 == 0 && s.t1 == tiles;
-  return s;
-}
+template <typename Requests>
+struct Walk {
+  const Extents& e;
+  const int32_t* start;
+  const Requests& requests;
+  int left;             // positions of the range that are left
+  int b, head, tile;    // the item, and the position within it
+  int at;
+  Request r;
 
-// The slots of a token's rows in request b's list, whose first tile is `start`: `in` gives those of one key
-// head, in ranges of `quota` tiles.
+  // the range [from, to) of the list, from < to
+  PAGED_CODE Walk(const Extents& e, const int32_t* start, const Requests& requests, int from, int to)
+      : e(e), start(start), requests(requests), left(to - from), b(find(start, e.requests + 1, from)), r(requests(b)) {
+    const int span = (start[b + 1] - start[b]) / e.kv;
+    at = from - start[b];
+    head = at / span;
+    at -= head * span;
+    tile = 0;
+    if (!r.narrow) {
+      int hi = row_tiles(e, r);  // the last row tile that begins at or before the position
+      while (hi - tile > 1) {
+        const int mid = (tile + hi) >> 1;
+        if (wide_begin(e, r, mid) <= at) tile = mid; else hi = mid;
+      }
+      at -= wide_begin(e, r, tile);
+    }
+  }
+  // the next segment; false at the end of the range
+  PAGED_CODE bool next(Segment& s) {
+    const int cost = r.narrow ? 0 : e.cost, skip = most(cost - at, 0);
+    if (left <= skip) return false;
+    const int tiles = item_tiles(e, r, tile);
+    s.head = head;
+    s.tile = tile;
+    s.t0 = at + skip - cost;
+    s.t1 = least(tiles, s.t0 + left - skip);
+    s.item = r.narrow ? narrow_item(e, b, head) : wide_item(e, r, b, head, tile);
+    s.all = s.t0 == 0 && s.t1 == tiles;
+    left -= skip + s.t1 - s.t0;
+    return true;
+  }
+  // past the item of the last segment, if the range goes on
+  PAGED_CODE void advance() {
+    if (left <= 0) return;
+    at = 0;
+    if (++tile < (r.narrow ? 1 : row_tiles(e, r))) return;
+    tile = 0;
+    if (++head < e.kv) return;
+    head = 0;
+    b = find(start, e.requests + 1, start[b + 1]);
+    r = requests(b);
+  }
+};
+
+// The slots of a token's rows in request b's list, whose first position is `start`: `in` gives those of one
+// key head, in ranges of `quota` positions.
 struct Slots {
   int first, count;
 };
 struct TokenSlots {
-  int t0, tiles, per_head;  // first key tile of the rows' item of key head 0, its tiles, tiles of a head
-  int item, items;          // that item, items of a head
-  int row;                  // the token's first row within a slot
+  int t0, tiles, span;  // position of the first key tile of the rows' item of key head 0, its tiles, positions of a head
+  int item, items;      // that item, items of a head
+  int row;              // the token's first row within a slot
   PAGED_CODE Slots in(int head, int quota) const {
     if (!tiles || !quota) return Slots{0, 0};
-    const int from = t0 + head * per_head, range = from / quota;
+    const int from = t0 + head * span, range = from / quota;
     return Slots{item + head * items + range, (from + tiles - 1) / quota - range + 1};
   }
 };
 PAGED_CODE TokenSlots token_slots(const Extents& e, const Request& r, int b, int start, int token) {
-  TokenSlots s{start, (int)head_tiles(e, r), 0, narrow_item(e, b, 0), 1, (token - r.first) * e.share};
-  s.per_head = s.tiles;
-  if (s.tiles && !r.narrow) {
-    const int i = token - r.first, tile = i / e.per, begin = (int)wide_tiles(e, r, tile);
-    s.tiles = (int)wide_tiles(e, r, tile + 1) - begin;
-    s.t0 += begin;
+  TokenSlots s{start, 0, 0, narrow_item(e, b, 0), 1, 0};
+  if (!r.count || !r.keys) return s;
+  const int i = token - r.first, tile = r.narrow ? 0 : i / e.per;
+  s.tiles = item_tiles(e, r, tile);
+  s.span = head_span(e, r);
+  if (!r.narrow) {
+    s.t0 += wide_begin(e, r, tile) + e.cost;
     s.item = wide_item(e, r, b, 0, tile);
     s.items = row_tiles(e, r);
-    s.row = (i - tile * e.per) * e.share;
   }
+  s.row = (i - (r.narrow ? 0 : tile * e.per)) * e.share;
   return s;
 }
 

@@ -28,13 +28,19 @@ struct Item { int list, b, head, tile; bool operator<(const Item& o) const {
   return list != o.list ? list < o.list : b != o.b ? b < o.b : head != o.head ? head < o.head : tile < o.tile; } };
 
 // 0, or the line that found a fault
-#define NEED(x) if (!(x)) return __LINE__
+#define NEED(...) if (!(__VA_ARGS__)) return __LINE__
 extern "C" int walk(int tokens, int requests, int heads, int kv, int shift, int columns, int prefix_columns, const int* offsets,
                     const int* lengths, int prefix_length, int monotone) {
-  const Extents e = extents(tokens, requests, heads, kv, shift, columns, prefix_columns);
+  Extents e = extents(tokens, requests, heads, kv, shift, columns, prefix_columns);
   auto request = [&](int b) {
     return b == requests ? prefix_request(e, offsets[b], prefix_length) : own_request(e, offsets[b], offsets[b + 1], lengths[b]);
   };
+  int64_t tiles = 0;
+  for (int b = 0; b <= requests; ++b) {
+    const Request r = request(b);
+    if (!r.narrow) tiles += (int64_t)kv * head_span(e, r);
+  }
+  e.cost = item_cost((int)tiles);
   std::vector<int32_t> starts[2];
   int64_t done[2] = {0, 0};
   for (int b = 0; b <= requests; ++b) {
@@ -42,7 +48,7 @@ extern "C" int walk(int tokens, int requests, int heads, int kv, int shift, int 
     NEED(r.first >= 0 && r.count >= 0 && r.first + r.count <= tokens);
     NEED(r.keys >= 0 && r.keys <= (int64_t)(r.prefix ? prefix_columns : columns) << shift);
     for (int k = 0; k < 2; ++k) starts[k].push_back(done[k]);
-    done[r.narrow] += (int64_t)kv * head_tiles(e, r);
+    done[r.narrow] += (int64_t)kv * head_span(e, r);
   }
   NEED(done[0] + done[1] + 2 * kStreams <= most_tiles(e) && most_tiles(e) < (int64_t)1 << 31);
   std::map<Item, std::vector<int64_t>> slots;  // slots of an item's segments, in order
@@ -55,24 +61,26 @@ extern "C" int walk(int tokens, int requests, int heads, int kv, int shift, int 
     quota[k] = (int)((done[k] + ranges - 1) / ranges);
     for (int range = 0; range < ranges; ++range) {
       const int64_t from = (int64_t)range * quota[k], to = from + quota[k] < done[k] ? from + quota[k] : done[k];
-      for (int64_t t = from; t < to;) {
-        const int b = find(starts[k].data(), requests + 1, (int)t);
-        const Request r = request(b);
-        NEED(r.narrow == (k == 1) && starts[k][b] <= t && t < starts[k][b + 1]);
-        const Segment s = segment_at(e, r, b, (starts[k][b + 1] - starts[k][b]) / kv, (int)t - starts[k][b], (int)(to - t));
-        NEED(s.head >= 0 && s.head < kv && s.tile >= 0 && s.t0 >= 0 && s.t1 > s.t0 && t + s.t1 - s.t0 <= to);
+      if (from >= to) continue;
+      Walk<decltype(request)> walk(e, starts[k].data(), request, (int)from, (int)to);
+      Segment s;
+      int taken = 0;
+      for (; walk.next(s); walk.advance()) {
+        const Request r = walk.r;
+        NEED(r.narrow == (k == 1) && s.head >= 0 && s.head < kv && s.tile >= 0 && s.t0 >= 0 && s.t1 > s.t0);
         NEED(r.narrow ? s.tile == 0 : s.tile < row_tiles(e, r));
+        NEED(s.t1 <= item_tiles(e, r, s.tile));
         const int64_t slot = s.item + range;
         NEED(slot >= 0 && slot < (k ? narrow_slots(e) : wide_slots(e)));
         if (monotone) NEED(used[k].insert(slot).second);
-        const Item item{k, b, s.head, s.tile};
+        const Item item{k, walk.b, s.head, s.tile};
         NEED(reached[item] == s.t0);
         reached[item] = s.t1;
         slots[item].push_back(slot);
-        NEED(s.all == (s.t0 == 0 && slots[item].size() == 1 && s.t1 == (r.narrow ? (int)head_tiles(e, r)
-             : (int)(wide_tiles(e, r, s.tile + 1) - wide_tiles(e, r, s.tile)))));
-        t += s.t1 - s.t0;
+        NEED(s.all == (slots[item].size() == 1 && s.t1 == item_tiles(e, r, s.tile)));
+        taken += s.t1 - s.t0;
       }
+      NEED(taken <= quota[k]);
     }
   }
   for (int b = 0; b <= requests; ++b) {
@@ -90,6 +98,9 @@ extern "C" int walk(int tokens, int requests, int heads, int kv, int shift, int 
         NEED(!rows.tiles || rows.row + share <= (k ? kNarrowRows : kWideRows));
         const auto& wrote = slots[Item{k, b, head, tile}];
         NEED(s.count == (int)wrote.size());
+        if (s.count) {
+          NEED(reached[Item{k, b, head, tile}] == rows.tiles);
+        }
         for (int n = 0; n < s.count; ++n) NEED(wrote[n] == s.first + n);
       }
   }
