@@ -44,10 +44,13 @@ __device__ inline Request request_of(const AttentionArgs& a, const Extents& e, i
                          : own_request(e, a.offsets[b], a.offsets[b + 1], a.lengths[b]);
 }
 
-__device__ __forceinline__ half4_t read_transposed(const _Float16* p) {
+template <typename T>
+__device__ __forceinline__ T read_lds(uint32_t at) {
+  return *(const T __attribute__((address_space(3)))*)(uintptr_t)at;
+}
+__device__ __forceinline__ half4_t read_transposed(uint32_t at) {
   typedef __fp16 fp16x4 __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
-      (fp16x4 __attribute__((address_space(3)))*)p));
+  return __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((fp16x4 __attribute__((address_space(3)))*)(uintptr_t)at));
 }
 
 __device__ __forceinline__ half8_t join(half4_t a, half4_t b) {
@@ -90,25 +93,31 @@ constexpr float kLazy = 8.0f;
 
 __device__ const uint4 zeros[1] = {};
 
-// 16 bytes a lane from global memory to LDS, lane l to dst + 16 l (dst the same in the whole wave).
+// 16 bytes a lane from global memory to LDS, lane l to dst + 16 l (dst, an LDS address, is the same in the whole wave).
 // Written as assembly: the compiler makes every LDS read wait for all such loads in flight, of
 // other buffers too; the waits here are written out where a stage is read.  (Nothing else here uses m0.)
-__device__ __forceinline__ void dma16(const void* src, const void* dst) {
-  const uint32_t at = (uint32_t)(uintptr_t)(const void __attribute__((address_space(3)))*)dst;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               :: "s"(uniform((int)at)), "v"(src) : "memory");
+__device__ __forceinline__ void dma16(const void* src, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(uniform((int)dst)), "v"(src) : "memory");
 }
-
-__device__ __forceinline__ void dma4(const void* src, const void* dst) {
-  const uint32_t at = (uint32_t)(uintptr_t)(const void __attribute__((address_space(3)))*)dst;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
-               :: "s"(uniform((int)at)), "v"(src) : "memory");
+__device__ __forceinline__ void dma4(const void* src, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(uniform((int)dst)), "v"(src) : "memory");
 }
-// 16 bytes with the part of the address that a wave shares in scalar registers.
-__device__ __forceinline__ void dma16(const void* base, uint32_t offset, const void* dst) {
-  const uint32_t at = (uint32_t)(uintptr_t)(const void __attribute__((address_space(3)))*)dst;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :: "s"(uniform((int)at)), "v"(offset), "s"(base) : "memory");
+// 16 rows of D values, one after another in memory from `base`, to LDS from dst on: D / 32 loads, which share the
+// scalar part of their addresses (the offset of an instruction counts on both sides).
+template <int D>
+__device__ __forceinline__ void dma_rows(const void* base, const uint32_t (&offset)[D / 32], uint32_t dst) {
+  if constexpr (D == 128)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
+                 "global_load_lds_dwordx4 %2, %5 offset:0x400\n\tglobal_load_lds_dwordx4 %3, %5 offset:0x800\n\t"
+                 "global_load_lds_dwordx4 %4, %5 offset:0xc00"
+                 :: "s"(uniform((int)dst)), "v"(offset[0]), "v"(offset[1]), "v"(offset[2]), "v"(offset[3]), "s"(base) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
+                 "global_load_lds_dwordx4 %2, %3 offset:0x400"
+                 :: "s"(uniform((int)dst)), "v"(offset[0]), "v"(offset[1]), "s"(base) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(const void __attribute__((address_space(3)))*)p;
 }
 
 // One key head of the cache behind a page list.  A wave holds a window of 64 entries of the list, one in
@@ -131,7 +140,7 @@ struct Keys {
   }
   __device__ __forceinline__ int entry(int index) const { return valid(index, list[min(index, last())]); }
   __device__ __forceinline__ void fetch(int from, int half) const {
-    dma4(list + min(from + lane, last()), ring + 64 * half);
+    dma4(list + min(from + lane, last()), lds_address(ring) + 256 * half);
   }
   __device__ __forceinline__ void open() {
     window = valid(first + lane, ring[64 * flip + lane]);
@@ -177,34 +186,39 @@ struct Keys {
   }
 };
 
-// This wave's rows of a tile: N loads of RPI rows each.  Whole tiles whose loads stay in one page have
-// their rows' offsets in scalar registers; others look each row up, and read zeros for a key that is not there.
-template <int D, int COUNT, int N>
+// A wave's rows of a tile, GROUPS times 16.  Where the tile is whole and pages hold 16 tokens or more, a group's
+// rows lie one after another, and where is in scalar registers; otherwise each row is looked up, and a key that
+// is not there read as zeros.
+template <int D, int COUNT, int GROUPS>
 struct Rows {
-  static constexpr int CH = D / 8, RPI = 512 / D;
-  size_t at[N];
+  static constexpr int CH = D / 8, RPI = 512 / D, PER = D / 32;  // chunks of a row, rows of a load, loads of a group
+  size_t at[GROUPS];
   bool fast;
   __device__ __forceinline__ void find(const Keys<D>& keys, int from, int r0) {
-    fast = (1 << keys.shift) >= RPI && keys.template whole<COUNT>(from);
+    fast = keys.shift >= 4 && keys.template whole<COUNT>(from);
     if (fast) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) at[n] = keys.row(from + r0 + n * RPI);
+      for (int g = 0; g < GROUPS; ++g) at[g] = keys.row(from + r0 + 16 * g);
     }
   }
   // lane_at: where a lane's 16 bytes are from the first of its load's rows
   __device__ __forceinline__ void load(const Keys<D>& keys, int from, int r0, const _Float16* matrix,
-                                       const uint32_t (&lane_at)[N], _Float16* dst) const {
+                                       const uint32_t (&lane_at)[PER], uint32_t dst) const {
     const int lane = keys.lane;
+    dst += 2 * r0 * D;
     if (fast) {
 #pragma unroll
-      for (int n = 0; n < N; ++n)
-        dma16(reinterpret_cast<const uint8_t*>(matrix) + at[n], lane_at[n], dst + (r0 + n * RPI) * D);
+      for (int g = 0; g < GROUPS; ++g)
+        dma_rows<D>(reinterpret_cast<const uint8_t*>(matrix) + at[g], lane_at, dst + 32 * g * D);
     } else {
+      int page[GROUPS * PER];
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const int key = from + r0 + n * RPI + lane / CH, p = keys.page(key);
-        const uint32_t chunk = lane_at[n] / 2 - (lane / CH) * D;
-        dma16(p < 0 ? (const void*)zeros : matrix + keys.at(p, key) + chunk, dst + (r0 + n * RPI) * D);
+      for (int n = 0; n < GROUPS * PER; ++n) page[n] = keys.page(from + r0 + n * RPI + lane / CH);
+#pragma unroll
+      for (int n = 0; n < GROUPS * PER; ++n) {
+        const int key = from + r0 + n * RPI + lane / CH;
+        const uint32_t chunk = lane_at[n % PER] / 2 - (lane / CH) * D;
+        dma16(page[n] < 0 ? (const void*)zeros : matrix + keys.at(page[n], key) + chunk, dst + 1024 * n);
       }
     }
   }
@@ -255,7 +269,7 @@ __device__ __forceinline__ half8_t pack8(const float* s) {
 template <int D>
 __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Extents& x, const Request& r, const Segment& seg,
                                              const int32_t* pages, float* slot, bool whole, _Float16* lds, int32_t* ring) {
-  constexpr int CH = D / 8, RPW = kWideKeys / kWaves, RPI = 512 / D, N = RPW / RPI;
+  constexpr int CH = D / 8, RPI = 512 / D, N = D / 32;  // chunks of a row, rows of a load, loads of this wave's 16 rows
   constexpr int MAT = kWideKeys * D;  // values of one staged matrix
   constexpr int DB = D / 32, AHEAD = 4;
   const int tid = here(), lane = tid & 63, wr = uniform(tid >> 6);
@@ -278,8 +292,9 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
     for (int kk = 0; kk < D / 16; ++kk) q[kk] = *reinterpret_cast<const half8_t*>(src + 16 * kk + 8 * half);
   }
   Keys<D> keys(a, seg.head, pages, bound, ring, lane);
-  using Tile = Rows<D, kWideKeys, N>;
-  const int r0 = wr * RPW;  // this wave loads 16 rows of a tile
+  static_assert(kWideKeys == 16 * kWaves, "a wave loads 16 rows of a tile");
+  using Tile = Rows<D, kWideKeys, 1>;
+  const int r0 = 16 * wr;
   uint32_t k_lane[N], v_lane[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
@@ -291,12 +306,23 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
   float m = -kInfinity, l = 0.0f, top;
   float s[16];  // scores, lane: row lane % 32, keys 8 (e / 4) + 4 half + e % 4
 
+  // LDS addresses of this lane's fragments: a row of K in the tile at hand, its chunks; and four rows of V^T for
+  // each 32 dimensions (a transposed read gives lane d of 16 four keys' values: rows of four, 16 dimensions of
+  // each).  The two places of a tile differ in one bit.
+  uint32_t k_at[D / 16], v_at[DB];
+  const uint32_t lds_at = lds_address(lds);
+#pragma unroll
+  for (int n = 0; n < D / 16; ++n) k_at[n] = lds_at + 2 * ((lane & 31) * D + 8 * key_chunk<D>(lane & 31, 2 * n + half));
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+    const int vr = 4 * half + ((lane & 15) >> 2);
+    v_at[db] = lds_at + 4 * MAT +
+               2 * (vr * D + 8 * value_chunk<D>(vr, 4 * db + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 4 * (lane & 1));
+  }
   // S^T = K Q^T of 32 keys, `between(n)` after each of its D / 16 products; fragment reads stay AHEAD of them
-  auto scores = [&](const _Float16* ks, auto between) {
-    auto fragment = [&](int n) {
-      const int kr = lane & 31;
-      return *reinterpret_cast<const half8_t*>(ks + kr * D + 8 * key_chunk<D>(kr, 2 * n + half));
-    };
+  auto scores = [&](auto half_tile, auto between) {
+    constexpr int AT = decltype(half_tile)::value * 64 * D;  // bytes
+    auto fragment = [&](int n) { return read_lds<half8_t>(k_at[n] + AT); };
     half8_t k[AHEAD];
     float16_t acc = {};
 #pragma unroll
@@ -333,19 +359,22 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
       for (int db = 0; db < DB; ++db) o[db] *= alpha;
     }
   };
-  // weights of the scores in s, with the scores of the next 32 keys (of ks) on the matrix cores meanwhile if
-  // NEXT; then O^T += V^T P^T for the 32 rows of values at vs, and the new scores' maximum meanwhile
-  auto advance = [&](auto next, const _Float16* ks, const _Float16* vs, int first, bool edge, uint32_t seen) {
+  // weights of the scores in s, made from half HALF of a tile, with the scores of the next 32 keys (half 1 - HALF of
+  // the tile that k_at is at) on the matrix cores meanwhile if NEXT; then O^T += V^T P^T, and the new scores'
+  // maximum meanwhile
+  auto advance = [&](auto next, auto half_tile, int first, bool edge, uint32_t seen) {
     constexpr bool NEXT = decltype(next)::value;
+    constexpr int HALF = decltype(half_tile)::value;
     const float mc = m == -kInfinity ? 0.0f : m * c;
     uint32_t p[8];
     auto weigh = [&](int i) {  // two scores to weights; the sum is of the weights as the product takes them
       const float2_t w = {__builtin_amdgcn_exp2f(s[2 * i] * c - mc), __builtin_amdgcn_exp2f(s[2 * i + 1] * c - mc)};
       p[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(w, half2_t));
       l = dot2(p[i], 0x3C003C00u, l);
+      asm volatile("" : "+v"(p[i]), "+v"(l));  // made here, not where they are used
     };
     if constexpr (NEXT) {
-      const float16_t acc = scores(ks, [&](int n) {
+      const float16_t acc = scores(std::integral_constant<int, 1 - HALF>{}, [&](int n) {
 #pragma unroll
         for (int i = 0; i < 128 / D; ++i) weigh(128 / D * n + i);
       });
@@ -354,12 +383,9 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
 #pragma unroll
       for (int i = 0; i < 8; ++i) weigh(i);
     }
-    // a transposed read gives lane d of 16 four keys' values: rows of four, 16 dimensions of each
     auto values = [&](int n) {
-      const int vr = 16 * (n / DB) + 4 * half + ((lane & 15) >> 2);
-      const int chunk = value_chunk<D>(vr, 4 * (n % DB) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1));
-      const _Float16* at = vs + vr * D + 8 * chunk + 4 * (lane & 1);
-      return join(read_transposed(at), read_transposed(at + 8 * D));
+      const uint32_t at = v_at[n % DB] + 2 * D * (32 * HALF + 16 * (n / DB));
+      return join(read_transposed(at), read_transposed(at + 16 * D));
     };
     half8_t v[AHEAD];
 #pragma unroll
@@ -384,7 +410,7 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
   const int safe = r.prefix ? r.keys : r.behind + seg.tile * x.per + 1;
   bool odd = false;
   // K of two tiles, V of two
-  auto place = [&](int t) { return lds + ((t - seg.t0) & 1) * MAT; };
+  auto place_at = [&](int t) { return lds_at + ((t - seg.t0) & 1) * 2 * MAT; };
   // A tile's way: its rows are found and its K loaded two tiles ahead, its V one.  `edge`: not all of it is seen by
   // all rows; `seen`: its keys that are there.
   Tile rows, rows1;
@@ -395,23 +421,27 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
     to.find(keys, from, r0);
     to_edge = from + kWideKeys > safe || !to.fast;
     to_seen = to.fast ? ~0ull : (uint64_t)__ballot(keys.page(from + lane) >= 0);
-    to.load(keys, from, r0, keys.k, k_lane, place(t));
+    to.load(keys, from, r0, keys.k, k_lane, place_at(t));
   };
-  auto load_v = [&](int t, const Tile& of) { of.load(keys, t * kWideKeys, r0, keys.v, v_lane, place(t) + 2 * MAT); };
+  auto load_v = [&](int t, const Tile& of) { of.load(keys, t * kWideKeys, r0, keys.v, v_lane, place_at(t) + 4 * MAT); };
   auto step = [&](int t, auto more1, auto more2) {  // of tiles t + 1 and t + 2
     constexpr bool MORE1 = decltype(more1)::value, MORE2 = decltype(more2)::value;
-    const _Float16 *ks = place(t), *vs = ks + 2 * MAT;
+    // of the two workgroups of a CU the older one's waves go first: the younger's take their turn every other tile
+    if (blockIdx.x >= kGroups / 2) {
+      if (t & 1) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(0);
+    }
     // V(t) has landed (K(t + 1) may be on its way), this wave's rows and after the barrier everyone's;
     // nobody reads V(t - 1) any more
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MORE1 ? N : 0) : "memory");
-    if ((t + 1) * kWideKeys > safe && !r.prefix) {
+    if (safe < bound && (t + 1) * kWideKeys > safe) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) odd |= clear_odd(place(t) + 2 * MAT + (r0 + n * RPI) * D + 8 * lane);
+      for (int n = 0; n < N; ++n) odd |= clear_odd(lds + ((t - seg.t0) & 1) * MAT + 2 * MAT + (r0 + n * RPI) * D + 8 * lane);
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if constexpr (MORE1) load_v(t + 1, rows1);
     if (wave_live) {
-      advance(std::true_type{}, ks + 32 * D, vs, t * kWideKeys + 32, edge, (uint32_t)(seen >> 32));
+      advance(std::true_type{}, std::integral_constant<int, 0>{}, t * kWideKeys + 32, edge, (uint32_t)(seen >> 32));
       rescale();
     }
     if constexpr (MORE1) {
@@ -425,7 +455,11 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
       find(t + 2, rows1, edge1, seen1);
     }
     if (wave_live) {
-      advance(more1, place(t + 1), vs + 32 * D, (t + 1) * kWideKeys, edge, (uint32_t)seen);
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) k_at[n] ^= 2 * MAT;
+      advance(more1, std::integral_constant<int, 1>{}, (t + 1) * kWideKeys, edge, (uint32_t)seen);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) v_at[db] ^= 2 * MAT;
       if constexpr (MORE1) rescale();
     }
   };
@@ -443,7 +477,7 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
   }
   if (wave_live) {
-    take(scores(place(seg.t0), [](int) {}), seg.t0 * kWideKeys, edge, (uint32_t)seen);
+    take(scores(std::integral_constant<int, 0>{}, [](int) {}), seg.t0 * kWideKeys, edge, (uint32_t)seen);
     top = s[0];
 #pragma unroll
     for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
@@ -456,6 +490,7 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
     ++t;
   }
   step(t, std::false_type{}, std::false_type{});
+  __builtin_amdgcn_s_setprio(0);
   l += __shfl_xor(l, 32);
   if (__syncthreads_or(odd)) {
     for (int key = max(seg.t0, max(safe, 0) / kWideKeys) * kWideKeys; key < min(seg.t1 * kWideKeys, bound); ++key) {
@@ -498,7 +533,7 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
 template <int D>
 __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Extents& x, const Request& r, const Segment& seg,
                                                const int32_t* pages, float* slot, bool whole, _Float16* lds, int32_t* ring) {
-  constexpr int CH = D / 8, RPI = 512 / D, N = kNarrowKeys / RPI, MAT = kNarrowKeys * D, DB = D / 16;
+  constexpr int CH = D / 8, RPI = 512 / D, PER = D / 32, N = 2 * PER, MAT = kNarrowKeys * D, DB = D / 16;
   const int lane = here() & 63, quad = lane >> 4, row = lane & 15;
   const int i = row / x.share, j = row - i * x.share;
   const bool live = i < r.count;
@@ -514,10 +549,10 @@ __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Ext
     for (int kk = 0; kk < D / 32; ++kk) q[kk] = *reinterpret_cast<const half8_t*>(src + 32 * kk + 8 * quad);
   }
   Keys<D> keys(a, seg.head, pages, bound, ring, lane);
-  using Tile = Rows<D, kNarrowKeys, N>;
-  uint32_t k_lane[N], v_lane[N];
+  using Tile = Rows<D, kNarrowKeys, 2>;
+  uint32_t k_lane[PER], v_lane[PER];
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
+  for (int n = 0; n < PER; ++n) {
     const int kr = n * RPI + lane / CH;
     k_lane[n] = 2 * ((lane / CH) * D + 8 * key_chunk<D>(kr, lane % CH));
     v_lane[n] = 2 * ((lane / CH) * D + 8 * value_chunk<D>(kr, lane % CH));
@@ -527,15 +562,16 @@ __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Ext
   bool odd = false;
   Tile rows;
   uint32_t seen, seen1 = 0;
+  const uint32_t lds_at = lds_address(lds);
   auto find = [&](int t, uint32_t& to_seen) {
     rows.find(keys, t * kNarrowKeys, 0);
     to_seen = rows.fast ? ~0u : (uint32_t)__ballot(keys.page(t * kNarrowKeys + (lane & 31)) >= 0);
-    rows.load(keys, t * kNarrowKeys, 0, keys.k, k_lane, lds);
+    rows.load(keys, t * kNarrowKeys, 0, keys.k, k_lane, lds_at);
   };
   keys.begin(seg.t0 * kNarrowKeys);
   settle(q);
   find(seg.t0, seen);
-  rows.load(keys, seg.t0 * kNarrowKeys, 0, keys.v, v_lane, lds + MAT);
+  rows.load(keys, seg.t0 * kNarrowKeys, 0, keys.v, v_lane, lds_at + 2 * MAT);
   for (int t = seg.t0; t < seg.t1; ++t) {
     const bool more = t + 1 < seg.t1;
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");  // K(t) has landed, V(t) is on its way
@@ -594,7 +630,7 @@ __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Ext
     // V(t) has landed, K(t + 1) is on its way
     if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (!r.prefix && first + kNarrowKeys > full) {  // keys that some row does not see
+    if (full < bound && first + kNarrowKeys > full) {  // keys that some row does not see
 #pragma unroll
       for (int n = 0; n < N; ++n) odd |= clear_odd(lds + MAT + n * RPI * D + 8 * lane);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -603,13 +639,13 @@ __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Ext
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
       const int vr = 4 * quad + (row >> 2), chunk = value_chunk<D>(vr, 2 * db + ((lane & 3) >> 1));
-      const _Float16* at = lds + MAT + vr * D + 8 * chunk + 4 * (lane & 1);
-      v[db] = join(read_transposed(at), read_transposed(at + 16 * D));
+      const uint32_t at = lds_at + 2 * (MAT + vr * D + 8 * chunk + 4 * (lane & 1));
+      v[db] = join(read_transposed(at), read_transposed(at + 32 * D));
     }
 #pragma unroll
     for (int db = 0; db < DB; ++db) o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[db], weight, o[db], 0, 0, 0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V(t) has been read
-    if (more) rows.load(keys, (t + 1) * kNarrowKeys, 0, keys.v, v_lane, lds + MAT);
+    if (more) rows.load(keys, (t + 1) * kNarrowKeys, 0, keys.v, v_lane, lds_at + 2 * MAT);
     seen = seen1;
   }
   l += __shfl_xor(l, 16);
@@ -647,6 +683,17 @@ __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Ext
   }
 }
 
+// Sum over the lanes up to this one: shifts within rows of 16, then the rows' totals.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast 31 into rows 2 and 3
+  return v;
+}
+
 // A token's rows in the slots of one list, as the joining kernel reads them: half a record.
 struct TokenPart {
   TokenSlots at;
@@ -658,32 +705,25 @@ static_assert(sizeof(TokenPart) == 2 * kRecord, "a record is two parts");
 // share of the wide tiles and each of its waves an equal share of the narrow ones.
 template <int D>
 __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
-  __shared__ __attribute__((aligned(16))) _Float16 tiles[kWaves * 8192];
+  __shared__ __attribute__((aligned(32768))) _Float16 tiles[kWaves * 8192];  // (the places of a tile differ in one bit)
   __shared__ __attribute__((aligned(16))) int32_t rings[kWaves][128];
   __shared__ int32_t starts[3][kAttentionMaxRequests + 2];
   __shared__ int32_t sums[3][kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   Extents x = extents_of(a);
   const int lists = a.requests + 1;
-  int done[3] = {0, 0, 0};  // tiles of the wide and the narrow list, items of the wide one
-  for (int base = 0; base < lists; base += kThreads) {
+  // tiles of the wide and the narrow list and items of the wide one, up to each request; the prefix comes last
+  int done[3] = {0, 0, 0};
+  const Request all = request_of(a, x, a.requests);
+  for (int base = 0; base < a.requests; base += kThreads) {
     const int b = base + tid;
-    int mine[3] = {0, 0, 0};
-    if (b < lists) {
-      const Request r = request_of(a, x, b);
-      const int span = a.kv * head_span(x, r);
-      mine[0] = r.narrow ? 0 : span;
-      mine[1] = r.narrow ? span : 0;
-      mine[2] = a.kv * head_items(x, r);
-    }
-    int scan[3] = {mine[0], mine[1], mine[2]};
+    const bool real = b < a.requests;
+    const Request r = request_of(a, x, min(b, a.requests - 1));
+    const int span = real ? a.kv * head_span(x, r) : 0;
+    const int mine[3] = {r.narrow ? 0 : span, r.narrow ? span : 0, real ? a.kv * head_items(x, r) : 0};
+    int scan[3];
 #pragma unroll
-    for (int step = 1; step < 64; step <<= 1)
-#pragma unroll
-      for (int k = 0; k < 3; ++k) {
-        const int below = __shfl_up(scan[k], step);
-        if (lane >= step) scan[k] += below;
-      }
+    for (int k = 0; k < 3; ++k) scan[k] = wave_scan(mine[k]);
     __syncthreads();
     if (lane == 63) {
 #pragma unroll
@@ -693,23 +733,34 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
       int before = done[k];
+#pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         if (w < wave) before += sums[k][w];
         done[k] += sums[k][w];
       }
-      if (b < lists) starts[k][b] = before + scan[k] - mine[k];
+      if (real) starts[k][b] = before + scan[k] - mine[k];
     }
   }
 #pragma unroll
   for (int k = 0; k < 3; ++k) done[k] = uniform(done[k]);
+  const int last[2] = {done[0], done[1]}, last_items = done[2];  // where the prefix begins
+  {
+    const int span = a.kv * head_span(x, all);
+    done[0] += all.narrow ? 0 : span;
+    done[1] += all.narrow ? span : 0;
+    done[2] += a.kv * head_items(x, all);
+  }
   x.cost = item_cost(done[0]);
   if (x.cost)  // each thread its own entries
-    for (int b = tid; b < lists; b += kThreads) starts[0][b] += x.cost * starts[2][b];
+    for (int b = tid; b < a.requests; b += kThreads) starts[0][b] += x.cost * starts[2][b];
   done[0] += x.cost * done[2];
-  if (tid < 2) starts[tid][lists] = tid ? done[1] : done[0];
+  if (tid < 2) {
+    starts[tid][a.requests] = tid ? last[1] : last[0] + x.cost * last_items;
+    starts[tid][lists] = tid ? done[1] : done[0];
+  }
   __syncthreads();
   const int quota[2] = {(done[0] + kGroups - 1) / kGroups, (done[1] + kStreams - 1) / kStreams};
-  const bool alone = prefix_request(x, a.tokens, *a.prefix_length).keys == 0;
+  const bool alone = all.keys == 0;
   float* const slots = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + record_bytes(a.tokens));
 
   const auto requests = [&](int b) { return request_of(a, x, b); };
@@ -755,27 +806,25 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
                         tiles + wave * 2 * kNarrowKeys * D, rings[wave]);
     }
   };
-  // The wide list is bound by arithmetic, the narrow one by memory: the second half of the workgroups, which
-  // share CUs with the first, takes them in the other order.
-  for (int turn = 0; turn < 2; ++turn) {
-    if ((blockIdx.x >= kGroups / 2) == (turn == 1)) wide_list();
-    else narrow_list();
-    __syncthreads();
-  }
+  wide_list();
+  __syncthreads();
+  narrow_list();
   // Where the joining kernel finds each token's slots, worked out by the last workgroups, which have the least
   // other work in small calls.
   for (int t = (kGroups - 1 - (int)blockIdx.x) * kThreads + tid; t < a.tokens; t += kGroups * kThreads) {
     TokenPart* record = static_cast<TokenPart*>(a.workspace) + 2 * (size_t)t;
-    const Request all = request_of(a, x, a.requests);
-    const int b = find(a.offsets, a.requests, t);
-    const Request r = request_of(a, x, b);
-    TokenPart shared{}, mine{};
-    if (t < all.count && t >= r.first && t < r.first + r.count) {
-      shared = TokenPart{token_slots(x, all, a.requests, starts[all.narrow][a.requests], t), all.narrow ? quota[1] : quota[0], all.narrow};
-      mine = TokenPart{token_slots(x, r, b, starts[r.narrow][b], t), r.narrow ? quota[1] : quota[0], r.narrow};
+    const int own = find(a.offsets, a.requests, t);
+    Request r = request_of(a, x, own);
+    const bool real = t < all.count && t >= r.first && t < r.first + r.count;
+#pragma unroll 1
+    for (int part = 1; part >= 0; --part) {  // its own list, the prefix's
+      TokenPart to{};
+      const int b = part ? own : a.requests;
+      if (real)
+        to = TokenPart{token_slots(x, r, b, starts[r.narrow][b], t), r.narrow ? quota[1] : quota[0], r.narrow};
+      record[part] = to;
+      r = all;
     }
-    record[0] = shared;
-    record[1] = mine;
   }
 }
 
