@@ -164,12 +164,13 @@ struct Keys {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     fetch(first + 64, flip ^ 1);
   }
-  // whether keys [from, from + COUNT), a tile of the window, are all there
+  // whether the tile of COUNT keys at `from`, in the window, has a key, and all the pages that it has keys in
   template <int COUNT>
   __device__ __forceinline__ bool whole(int from) const {
-    const int entries = COUNT >> shift > 1 ? COUNT >> shift : 1;  // at most 64
-    const uint64_t want = (entries == 64 ? 0 : 1ull << entries) - 1;
-    return from + COUNT <= bound && !(want & ~(there >> ((from >> shift) - first)));
+    if (from >= bound) return false;  // (where a request's first tokens see nothing)
+    const int at = (from >> shift) - first, entries = min((from + COUNT - 1) >> shift, last()) - first - at + 1;  // 1 to 64
+    const uint64_t want = entries >= 64 ? ~0ull : (1ull << entries) - 1;
+    return !(want & ~(there >> at));
   }
   // the page of a key of the window, -1 for none
   __device__ __forceinline__ int page(int key) const {
@@ -186,9 +187,10 @@ struct Keys {
   }
 };
 
-// A wave's rows of a tile, GROUPS times 16.  Where the tile is whole and pages hold 16 tokens or more, a group's
-// rows lie one after another, and where is in scalar registers; otherwise each row is looked up, and a key that
-// is not there read as zeros.
+// A wave's rows of a tile, GROUPS times 16.  Where all its pages are there and hold 16 tokens or more, a group's
+// rows lie one after another, and where is in scalar registers (those of a page that are past the last key are
+// loaded too; a group past it is the last one again).  Otherwise each row is looked up, and a key that is not there
+// read as zeros.
 template <int D, int COUNT, int GROUPS>
 struct Rows {
   static constexpr int CH = D / 8, RPI = 512 / D, PER = D / 32;  // chunks of a row, rows of a load, loads of a group
@@ -198,7 +200,7 @@ struct Rows {
     fast = keys.shift >= 4 && keys.template whole<COUNT>(from);
     if (fast) {
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) at[g] = keys.row(from + r0 + 16 * g);
+      for (int g = 0; g < GROUPS; ++g) at[g] = keys.row(min(from + r0 + 16 * g, (keys.bound - 1) & ~15));
     }
   }
   // lane_at: where a lane's 16 bytes are from the first of its load's rows
@@ -232,6 +234,15 @@ __device__ __forceinline__ bool raise(float top, float& m, float& alpha, float c
   alpha = m == -kInfinity ? 0.0f : exp2f((m - next) * c);
   m = next;
   return true;
+}
+
+// The weights of keys past the last one are 0, and so must be their values: this lane's rows of a staged tile,
+// RPI rows apart from `key` on.
+template <int D, int N>
+__device__ __forceinline__ void clear_past(_Float16* at, int key, int bound) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    if (key + n * (512 / D) >= bound) *reinterpret_cast<uint4*>(at + 512 * n) = uint4{};
 }
 
 // Where some rows of a tile do not see a key, its weight of 0 would still turn a value that is not
@@ -434,9 +445,11 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
     // V(t) has landed (K(t + 1) may be on its way), this wave's rows and after the barrier everyone's;
     // nobody reads V(t - 1) any more
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MORE1 ? N : 0) : "memory");
+    _Float16* const mine = lds + ((t - seg.t0) & 1) * MAT + 2 * MAT + r0 * D + 8 * lane;
+    if ((t + 1) * kWideKeys > bound) clear_past<D, N>(mine, t * kWideKeys + r0 + lane / CH, bound);
     if (safe < bound && (t + 1) * kWideKeys > safe) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) odd |= clear_odd(lds + ((t - seg.t0) & 1) * MAT + 2 * MAT + (r0 + n * RPI) * D + 8 * lane);
+      for (int n = 0; n < N; ++n) odd |= clear_odd(mine + n * 512);
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if constexpr (MORE1) load_v(t + 1, rows1);
@@ -630,9 +643,12 @@ __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Ext
     // V(t) has landed, K(t + 1) is on its way
     if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (full < bound && first + kNarrowKeys > full) {  // keys that some row does not see
+    if (first + kNarrowKeys > full) {  // keys that some row does not see, or past the last
+      if (first + kNarrowKeys > bound) clear_past<D, N>(lds + MAT + 8 * lane, first + lane / CH, bound);
+      if (full < bound) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) odd |= clear_odd(lds + MAT + n * RPI * D + 8 * lane);
+        for (int n = 0; n < N; ++n) odd |= clear_odd(lds + MAT + n * 512 + 8 * lane);
+      }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     half8_t v[DB];
