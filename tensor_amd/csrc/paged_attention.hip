@@ -276,10 +276,11 @@ __device__ __forceinline__ half8_t pack8(const float* s) {
   return __builtin_bit_cast(half8_t, v);
 }
 
-// One segment of a wide item: up to 128 rows, 32 a wave, against key tiles [t0, t1).
+// One segment of a wide item: up to 128 rows, 32 a wave, against key tiles [t0, t1), of which the first x.lead of
+// a request are the shared prefix's.
 template <int D>
 __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Extents& x, const Request& r, const Segment& seg,
-                                             const int32_t* pages, float* slot, bool whole, _Float16* lds, int32_t* ring) {
+                                             const int32_t* pages, int prefix_keys, float* slot, bool whole, _Float16* lds, int32_t* ring) {
   constexpr int CH = D / 8, RPI = 512 / D, N = D / 32;  // chunks of a row, rows of a load, loads of this wave's 16 rows
   constexpr int MAT = kWideKeys * D;  // values of one staged matrix
   constexpr int DB = D / 32, AHEAD = 4;
@@ -289,10 +290,7 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
   const bool live = ti < x.per && i < r.count;
   const int ti_first = uniform(wr * 32 / x.share), i_first = seg.tile * x.per + ti_first;
   const bool wave_live = ti_first < x.per && i_first < r.count;
-  const int i_last = min(r.count, (seg.tile + 1) * x.per) - 1;
-  const int bound = r.prefix ? r.keys : min(r.keys, r.behind + i_last + 1);
-  const int limit = r.prefix ? r.keys : r.behind + (live ? i : i_first) + 1;
-  const int full = r.prefix ? r.keys : r.behind + i_first + 1;  // keys that every row of this wave sees
+  const int i_last = min(r.count, (seg.tile + 1) * x.per) - 1, lead = lead_of(x, r);
   const float c = a.scale * 1.44269504088896340736f;
 
   half8_t q[D / 16];
@@ -302,7 +300,6 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) q[kk] = *reinterpret_cast<const half8_t*>(src + 16 * kk + 8 * half);
   }
-  Keys<D> keys(a, seg.head, pages, bound, ring, lane);
   static_assert(kWideKeys == 16 * kWaves, "a wave loads 16 rows of a tile");
   using Tile = Rows<D, kWideKeys, 1>;
   const int r0 = 16 * wr;
@@ -322,14 +319,16 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
   // each).  The two places of a tile differ in one bit.
   uint32_t k_at[D / 16], v_at[DB];
   const uint32_t lds_at = lds_address(lds);
+  auto first_place = [&]() {
 #pragma unroll
-  for (int n = 0; n < D / 16; ++n) k_at[n] = lds_at + 2 * ((lane & 31) * D + 8 * key_chunk<D>(lane & 31, 2 * n + half));
+    for (int n = 0; n < D / 16; ++n) k_at[n] = lds_at + 2 * ((lane & 31) * D + 8 * key_chunk<D>(lane & 31, 2 * n + half));
 #pragma unroll
-  for (int db = 0; db < DB; ++db) {
-    const int vr = 4 * half + ((lane & 15) >> 2);
-    v_at[db] = lds_at + 4 * MAT +
-               2 * (vr * D + 8 * value_chunk<D>(vr, 4 * db + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 4 * (lane & 1));
-  }
+    for (int db = 0; db < DB; ++db) {
+      const int vr = 4 * half + ((lane & 15) >> 2);
+      v_at[db] = lds_at + 4 * MAT +
+                 2 * (vr * D + 8 * value_chunk<D>(vr, 4 * db + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 4 * (lane & 1));
+    }
+  };
   // S^T = K Q^T of 32 keys, `between(n)` after each of its D / 16 products; fragment reads stay AHEAD of them
   auto scores = [&](auto half_tile, auto between) {
     constexpr int AT = decltype(half_tile)::value * 64 * D;  // bytes
@@ -349,6 +348,7 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
     return acc;
   };
   // the scores of keys [first, first + 32); edge: some may not be seen by some row
+  int limit;  // this row's keys of the list at hand
   auto take = [&](const float16_t& acc, int first, bool edge, uint32_t seen) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[e] = acc[e];
@@ -417,110 +417,120 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  // Tiles up to `safe` are seen whole by every row of the workgroup.
-  const int safe = r.prefix ? r.keys : r.behind + seg.tile * x.per + 1;
-  bool odd = false;
-  // K of two tiles, V of two
-  auto place_at = [&](int t) { return lds_at + ((t - seg.t0) & 1) * 2 * MAT; };
-  // A tile's way: its rows are found and its K loaded two tiles ahead, its V one.  `edge`: not all of it is seen by
-  // all rows; `seen`: its keys that are there.
-  Tile rows, rows1;
-  bool edge, edge1 = false;
-  uint64_t seen, seen1 = 0;
-  auto find = [&](int t, Tile& to, bool& to_edge, uint64_t& to_seen) {
-    const int from = t * kWideKeys;
-    to.find(keys, from, r0);
-    to_edge = from + kWideKeys > safe || !to.fast;
-    to_seen = to.fast ? ~0ull : (uint64_t)__ballot(keys.page(from + lane) >= 0);
-    to.load(keys, from, r0, keys.k, k_lane, place_at(t));
-  };
-  auto load_v = [&](int t, const Tile& of) { of.load(keys, t * kWideKeys, r0, keys.v, v_lane, place_at(t) + 4 * MAT); };
-  auto step = [&](int t, auto more1, auto more2) {  // of tiles t + 1 and t + 2
-    constexpr bool MORE1 = decltype(more1)::value, MORE2 = decltype(more2)::value;
-    // of the two workgroups of a CU the older one's waves go first: the younger's take their turn every other tile
-    if (blockIdx.x >= kGroups / 2) {
-      if (t & 1) __builtin_amdgcn_s_setprio(1);
-      else __builtin_amdgcn_s_setprio(0);
-    }
-    // V(t) has landed (K(t + 1) may be on its way), this wave's rows and after the barrier everyone's;
-    // nobody reads V(t - 1) any more
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MORE1 ? N : 0) : "memory");
-    _Float16* const mine = lds + ((t - seg.t0) & 1) * MAT + 2 * MAT + r0 * D + 8 * lane;
-    if ((t + 1) * kWideKeys > bound) clear_past<D, N>(mine, t * kWideKeys + r0 + lane / CH, bound);
-    if (safe < bound && (t + 1) * kWideKeys > safe) {
+#pragma unroll 1
+  for (int from = seg.t0; from < seg.t1;) {  // the prefix's keys, the request's own
+    const bool shared = r.prefix || from < lead;
+    const int own = r.prefix || shared ? 0 : lead, t0 = from - own, t1 = (from < lead ? min(seg.t1, lead) : seg.t1) - own;
+    from = t1 + own;
+    const int bound = shared ? prefix_keys : min(r.keys, r.behind + i_last + 1);
+    limit = shared ? prefix_keys : r.behind + (live ? i : i_first) + 1;
+    Keys<D> keys(a, seg.head, shared ? a.prefix_pages : pages, bound, ring, lane);
+    // Tiles up to `safe` are seen whole by every row of the workgroup.
+    const int safe = shared ? bound : r.behind + seg.tile * x.per + 1;
+    bool odd = false;
+    // K of two tiles, V of two
+    auto place_at = [&](int t) { return lds_at + ((t - t0) & 1) * 2 * MAT; };
+    // A tile's way: its rows are found and its K loaded two tiles ahead, its V one.  `edge`: not all of it is seen by
+    // all rows; `seen`: its keys that are there.
+    Tile rows, rows1;
+    bool edge, edge1 = false;
+    uint64_t seen, seen1 = 0;
+    auto find = [&](int t, Tile& to, bool& to_edge, uint64_t& to_seen) {
+      const int from = t * kWideKeys;
+      to.find(keys, from, r0);
+      to_edge = from + kWideKeys > safe || !to.fast;
+      to_seen = to.fast ? ~0ull : (uint64_t)__ballot(keys.page(from + lane) >= 0);
+      to.load(keys, from, r0, keys.k, k_lane, place_at(t));
+    };
+    auto load_v = [&](int t, const Tile& of) { of.load(keys, t * kWideKeys, r0, keys.v, v_lane, place_at(t) + 4 * MAT); };
+    auto step = [&](int t, auto more1, auto more2) {  // of tiles t + 1 and t + 2
+      constexpr bool MORE1 = decltype(more1)::value, MORE2 = decltype(more2)::value;
+      // of the two workgroups of a CU the older one's waves go first: the younger's take their turn every other tile
+      if (blockIdx.x >= kGroups / 2) {
+        if (t & 1) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+      }
+      // V(t) has landed (K(t + 1) may be on its way), this wave's rows and after the barrier everyone's;
+      // nobody reads V(t - 1) any more
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MORE1 ? N : 0) : "memory");
+      _Float16* const mine = lds + ((t - t0) & 1) * MAT + 2 * MAT + r0 * D + 8 * lane;
+      if ((t + 1) * kWideKeys > bound) clear_past<D, N>(mine, t * kWideKeys + r0 + lane / CH, bound);
+      if (safe < bound && (t + 1) * kWideKeys > safe) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) odd |= clear_odd(mine + n * 512);
+        for (int n = 0; n < N; ++n) odd |= clear_odd(mine + n * 512);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if constexpr (MORE1) load_v(t + 1, rows1);
+      if (wave_live) {
+        advance(std::true_type{}, std::integral_constant<int, 0>{}, t * kWideKeys + 32, edge, (uint32_t)(seen >> 32));
+        rescale();
+      }
+      if constexpr (MORE1) {
+        // the same of K(t + 1), V(t + 1) and K(t)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+      }
+      edge = edge1;
+      seen = seen1;
+      if constexpr (MORE2) {
+        keys.reach((t + 2) * kWideKeys);
+        find(t + 2, rows1, edge1, seen1);
+      }
+      if (wave_live) {
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) k_at[n] ^= 2 * MAT;
+        advance(more1, std::integral_constant<int, 1>{}, (t + 1) * kWideKeys, edge, (uint32_t)seen);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) v_at[db] ^= 2 * MAT;
+        if constexpr (MORE1) rescale();
+      }
+    };
+
+    keys.begin(t0 * kWideKeys);
+    settle(q);
+    first_place();
+    __syncthreads();  // the tiles' places are free
+    find(t0, rows, edge, seen);
+    load_v(t0, rows);
+    if (t0 + 1 < t1) {
+      keys.reach((t0 + 1) * kWideKeys);
+      find(t0 + 1, rows1, edge1, seen1);
+      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * N) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
     }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if constexpr (MORE1) load_v(t + 1, rows1);
     if (wave_live) {
-      advance(std::true_type{}, std::integral_constant<int, 0>{}, t * kWideKeys + 32, edge, (uint32_t)(seen >> 32));
+      take(scores(std::integral_constant<int, 0>{}, [](int) {}), t0 * kWideKeys, edge, (uint32_t)seen);
+      top = s[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
       rescale();
     }
-    if constexpr (MORE1) {
-      // the same of K(t + 1), V(t + 1) and K(t)
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+    int t = t0;
+    for (; t + 2 < t1; ++t) step(t, std::true_type{}, std::true_type{});
+    if (t + 1 < t1) {
+      step(t, std::true_type{}, std::false_type{});
+      ++t;
     }
-    edge = edge1;
-    seen = seen1;
-    if constexpr (MORE2) {
-      keys.reach((t + 2) * kWideKeys);
-      find(t + 2, rows1, edge1, seen1);
+    step(t, std::false_type{}, std::false_type{});
+    __builtin_amdgcn_s_setprio(0);
+    if (__syncthreads_or(odd)) {
+      for (int key = max(t0, max(safe, 0) / kWideKeys) * kWideKeys; key < min(t1 * kWideKeys, bound); ++key) {
+        const int page = keys.entry(key >> x.page_shift);
+        if (page < 0 || key >= limit) continue;
+        const _Float16* v = keys.v + keys.at(page, key) + 4 * half;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float part[4] = {o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+            add_odd(*reinterpret_cast<const half4_t*>(v + 32 * db + 8 * g), part);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[db][4 * g + e] = part[e];
+          }
+      }
     }
-    if (wave_live) {
-#pragma unroll
-      for (int n = 0; n < D / 16; ++n) k_at[n] ^= 2 * MAT;
-      advance(more1, std::integral_constant<int, 1>{}, (t + 1) * kWideKeys, edge, (uint32_t)seen);
-#pragma unroll
-      for (int db = 0; db < DB; ++db) v_at[db] ^= 2 * MAT;
-      if constexpr (MORE1) rescale();
-    }
-  };
-
-  keys.begin(seg.t0 * kWideKeys);
-  settle(q);
-  __syncthreads();  // the tiles' places are free
-  find(seg.t0, rows, edge, seen);
-  load_v(seg.t0, rows);
-  if (seg.t0 + 1 < seg.t1) {
-    keys.reach((seg.t0 + 1) * kWideKeys);
-    find(seg.t0 + 1, rows1, edge1, seen1);
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * N) : "memory");
-  } else {
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
   }
-  if (wave_live) {
-    take(scores(std::integral_constant<int, 0>{}, [](int) {}), seg.t0 * kWideKeys, edge, (uint32_t)seen);
-    top = s[0];
-#pragma unroll
-    for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-    rescale();
-  }
-  int t = seg.t0;
-  for (; t + 2 < seg.t1; ++t) step(t, std::true_type{}, std::true_type{});
-  if (t + 1 < seg.t1) {
-    step(t, std::true_type{}, std::false_type{});
-    ++t;
-  }
-  step(t, std::false_type{}, std::false_type{});
-  __builtin_amdgcn_s_setprio(0);
   l += __shfl_xor(l, 32);
-  if (__syncthreads_or(odd)) {
-    for (int key = max(seg.t0, max(safe, 0) / kWideKeys) * kWideKeys; key < min(seg.t1 * kWideKeys, bound); ++key) {
-      const int page = keys.entry(key >> x.page_shift);
-      if (page < 0 || key >= limit) continue;
-      const _Float16* v = keys.v + keys.at(page, key) + 4 * half;
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float part[4] = {o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
-          add_odd(*reinterpret_cast<const half4_t*>(v + 32 * db + 8 * g), part);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[db][4 * g + e] = part[e];
-        }
-    }
-  }
   if (!live) return;
   const float norm = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -724,19 +734,22 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
   __shared__ __attribute__((aligned(32768))) _Float16 tiles[kWaves * 8192];  // (the places of a tile differ in one bit)
   __shared__ __attribute__((aligned(16))) int32_t rings[kWaves][128];
   __shared__ int32_t starts[3][kAttentionMaxRequests + 2];
-  __shared__ int32_t sums[3][kWaves];
+  __shared__ int32_t sums[4][kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   Extents x = extents_of(a);
   const int lists = a.requests + 1;
   // tiles of the wide and the narrow list and items of the wide one, up to each request; the prefix comes last
   int done[3] = {0, 0, 0};
-  const Request all = request_of(a, x, a.requests);
+  Request all = request_of(a, x, a.requests);
+  const int tokens = all.count;
+  bool apart = false, broken = false;  // narrow requests, or ones without keys; offsets that do not ascend
   for (int base = 0; base < a.requests; base += kThreads) {
     const int b = base + tid;
     const bool real = b < a.requests;
     const Request r = request_of(a, x, min(b, a.requests - 1));
     const int span = real ? a.kv * head_span(x, r) : 0;
     const int mine[3] = {r.narrow ? 0 : span, r.narrow ? span : 0, real ? a.kv * head_items(x, r) : 0};
+    const bool odd[2] = {(bool)__any(real && r.count && (r.narrow || !r.keys)), (bool)__any(real && a.offsets[b] > a.offsets[b + 1])};
     int scan[3];
 #pragma unroll
     for (int k = 0; k < 3; ++k) scan[k] = wave_scan(mine[k]);
@@ -744,6 +757,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
     if (lane == 63) {
 #pragma unroll
       for (int k = 0; k < 3; ++k) sums[k][wave] = scan[k];
+      sums[3][wave] = odd[0] | odd[1] << 1;
     }
     __syncthreads();
 #pragma unroll
@@ -756,9 +770,18 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
       }
       if (real) starts[k][b] = before + scan[k] - mine[k];
     }
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      apart |= sums[3][w] & 1;
+      broken |= sums[3][w] >> 1;
+    }
   }
 #pragma unroll
   for (int k = 0; k < 3; ++k) done[k] = uniform(done[k]);
+  const int prefix_keys = uniform(all.keys);
+  x.lead = uniform(apart ? 0 : lead_tiles(x, all, done[2] / a.kv));
+  if (x.lead) all.count = all.keys = 0;  // each request's items take it
+  done[0] += x.lead * done[2];
   const int last[2] = {done[0], done[1]}, last_items = done[2];  // where the prefix begins
   {
     const int span = a.kv * head_span(x, all);
@@ -767,9 +790,10 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
     done[2] += a.kv * head_items(x, all);
   }
   x.cost = item_cost(done[0]);
-  if (x.cost)  // each thread its own entries
-    for (int b = tid; b < a.requests; b += kThreads) starts[0][b] += x.cost * starts[2][b];
+  if (x.cost + x.lead)  // each thread its own entries
+    for (int b = tid; b < a.requests; b += kThreads) starts[0][b] += (x.cost + x.lead) * starts[2][b];
   done[0] += x.cost * done[2];
+  if (uniform(broken)) done[0] = done[1] = 0;  // their sums may not hold: no row sees anything
   if (tid < 2) {
     starts[tid][a.requests] = tid ? last[1] : last[0] + x.cost * last_items;
     starts[tid][lists] = tid ? done[1] : done[0];
@@ -804,7 +828,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
     Walk<decltype(requests)> walk(x, starts[0], requests, range * quota[0], min((range + 1) * quota[0], done[0]));
     Segment seg;
     for (settle(walk); walk.next(seg); walk.advance(), settle(walk)) {
-      wide_segment<D>(a, x, walk.r, seg, list_of(walk.r, walk.b),
+      wide_segment<D>(a, x, walk.r, seg, list_of(walk.r, walk.b), prefix_keys,
                       slots + slot_floats(kWideRows, D) * (size_t)(seg.item + range), alone && !walk.r.prefix && seg.all,
                       tiles, rings[wave]);
     }
@@ -831,7 +855,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
     TokenPart* record = static_cast<TokenPart*>(a.workspace) + 2 * (size_t)t;
     const int own = find(a.offsets, a.requests, t);
     Request r = request_of(a, x, own);
-    const bool real = t < all.count && t >= r.first && t < r.first + r.count;
+    const bool real = t < tokens && t >= r.first && t < r.first + r.count;
 #pragma unroll 1
     for (int part = 1; part >= 0; --part) {  // its own list, the prefix's
       TokenPart to{};
@@ -850,7 +874,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
 // weight for all dimensions and the outputs' loads wait for nothing but the record.
 template <int D, int THREADS>
 __global__ __launch_bounds__(THREADS) void join_segments(const AttentionArgs a, int split) {
-  constexpr int LANES = D / 4, SETS = THREADS / LANES, BATCH = 8;
+  constexpr int LANES = D / 4, SETS = THREADS / LANES, BATCH = 4;
   const int tid = threadIdx.x, lane = tid % LANES, set = tid / LANES, part = set % split;
   const int per = SETS / split, rows_all = a.tokens * a.heads, row = blockIdx.x * per + set / split;
   const Extents x = extents_of(a);
@@ -873,7 +897,9 @@ __global__ __launch_bounds__(THREADS) void join_segments(const AttentionArgs a, 
     sum_at[k] = rows;
     out_at[k] = 2 * rows + at * (D - 1) + 4 * lane;
   }
-  const int all = count[0] + count[1];
+  // rows whose only segment wrote the output itself
+  const bool done = row >= rows_all || (count[1] == 1 && parts[0].at.tiles == 0);
+  const int all = done ? 0 : count[0] + count[1];
   auto slot = [&](int p, bool k) { return from[k] + stride[k] * (size_t)(k ? p - count[0] : p); };
   // over the lanes of a set
   auto highest = [&](float v) {
@@ -931,8 +957,7 @@ __global__ __launch_bounds__(THREADS) void join_segments(const AttentionArgs a, 
     o = float4_t{};
     for (int s = 0; s < split; ++s) o += outs[tid + s * LANES] * __shfl(w, s, LANES);
   }
-  // rows whose only segment wrote the output itself
-  if (row >= rows_all || (count[1] == 1 && parts[0].at.tiles == 0)) return;
+  if (done) return;
   const float4_t v = o * (l == 0.0f ? 0.0f : 1.0f / l);
   *reinterpret_cast<uint2*>(static_cast<_Float16*>(a.out) + (size_t)row * D + 4 * lane) =
       make_uint2(half2_from_fp32(v[0], v[1]), half2_from_fp32(v[2], v[3]));

@@ -10,6 +10,10 @@
 // Slot = item + range: both only grow along the list, one of them with every segment.  To begin a wide item
 // costs a workgroup as much as kItemCost tiles, so in long lists each has that many empty positions before its
 // first tile (in short ones a range of one more tile would cost more than it evens out).
+//
+// The prefix is a list entry of its own where tokens of several requests fill its row tiles; where each request
+// fills tiles of its own (prompts, one request), its wide items begin with the prefix's tiles instead (`lead`),
+// which leaves one slot less to write and join.
 #pragma once
 
 #include <stddef.h>
@@ -28,6 +32,7 @@ constexpr int kGroups = 512;                // workgroups: two per CU
 constexpr int kStreams = kGroups * kWaves;  // waves of the launch
 constexpr int kWideRows = 128, kWideKeys = 64, kNarrowRows = 16, kNarrowKeys = 32;
 constexpr int kItemCost = 3, kLongRange = 24;  // tiles of a range from which items have a cost
+constexpr int kSlotCost = 8;                   // to begin an item, leave its rows in a slot and join them, in tiles
 
 PAGED_CODE int least(int a, int b) { return a < b ? a : b; }
 PAGED_CODE int most(int a, int b) { return a > b ? a : b; }
@@ -36,11 +41,12 @@ PAGED_CODE int most(int a, int b) { return a > b ? a : b; }
 struct Extents {
   int tokens, requests, kv, share, page_shift, columns, prefix_columns;  // share: query heads of a key head
   int per;                                                               // tokens of a wide row tile
-  int cost;                                                              // positions before an item's first tile
+  int cost;                                                              // positions before a wide item's first tile
+  int lead;                                                              // tiles of the prefix, of which its requests' items consist first
 };
 PAGED_CODE Extents extents(int tokens, int requests, int heads, int kv, int page_shift, int columns, int prefix_columns) {
   const int share = heads / kv;
-  return Extents{tokens, requests, kv, share, page_shift, columns, prefix_columns, kWideRows / share, 0};
+  return Extents{tokens, requests, kv, share, page_shift, columns, prefix_columns, kWideRows / share, 0, 0};
 }
 
 // Workspace: a record of each token for the joining kernel, then wide and narrow slots.
@@ -124,23 +130,31 @@ PAGED_CODE int64_t most_tiles(const Extents& e) {
   return e.kv * (e.tokens / e.per * 2 + e.requests + 3ll) * ((keys + e.tokens) / kNarrowKeys + 2 + kItemCost) + 2 * kStreams;
 }
 
-// Positions of one key head in its list: key tiles, and a wide item's cost.
+PAGED_CODE int lead_of(const Extents& e, const Request& r) { return r.prefix ? 0 : e.lead; }
+// Where row tile `tile` of a wide request begins within its key head's positions: key tiles, and items' costs.
+PAGED_CODE int wide_begin(const Extents& e, const Request& r, int tile) {
+  return (int)wide_tiles(e, r, tile) + (e.cost + lead_of(e, r)) * tile;
+}
+// Positions of one key head in its list.
 PAGED_CODE int head_span(const Extents& e, const Request& r) {
   if (!r.count || !r.keys) return 0;
   if (r.narrow) return (r.keys + kNarrowKeys - 1) / kNarrowKeys;
-  return (int)wide_tiles(e, r, row_tiles(e, r)) + e.cost * row_tiles(e, r);
+  return wide_begin(e, r, row_tiles(e, r));
 }
 // Items of one key head in the wide list.
 PAGED_CODE int head_items(const Extents& e, const Request& r) { return r.count && r.keys && !r.narrow ? row_tiles(e, r) : 0; }
 PAGED_CODE int item_cost(int tiles) { return tiles >= kLongRange * kGroups ? kItemCost : 0; }  // by the wide list's tiles
-// Where row tile `tile` of a wide request begins within its key head, and the key tiles of a row tile.
-PAGED_CODE int wide_begin(const Extents& e, const Request& r, int tile) {
-  return (int)wide_tiles(e, r, tile) + e.cost * tile;
-}
+// Key tiles of a row tile.
 PAGED_CODE int item_tiles(const Extents& e, const Request& r, int tile) {
   if (r.narrow) return (r.keys + kNarrowKeys - 1) / kNarrowKeys;
   const int keys = r.prefix ? r.keys : most(r.behind, 0) + least(r.count, (tile + 1) * e.per);
-  return (keys + kWideKeys - 1) / kWideKeys;
+  return lead_of(e, r) + (keys + kWideKeys - 1) / kWideKeys;
+}
+// The prefix's tiles if they are to lead `items` wide items (of one key head), all that the requests have; else 0.
+// That costs the tiles that more items than the prefix's own have, and saves the latter.
+PAGED_CODE int lead_tiles(const Extents& e, const Request& prefix, int items) {
+  const int tiles = prefix.count ? (prefix.keys + kWideKeys - 1) / kWideKeys : 0, own = row_tiles(e, prefix);
+  return !prefix.narrow && (int64_t)(items - own) * tiles <= (int64_t)own * kSlotCost ? tiles : 0;
 }
 
 // Items of request b (b = requests: the prefix) grow along the list and stay within the slots.

@@ -278,6 +278,26 @@ def test_attention_of_many_tokens(hip_device, heads, dim):
         assert (run_attention(hip_device, *call)[-3:] == 0).all()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("counts,lengths", [([40], [40]), ([33, 0, 64, 130], [50, 7, 64, 300]), ([90, 5, 64], [90, 0, 9])], ids=str)
+def test_attention_of_prompts_behind_a_prefix(hip_device, counts, lengths, dim):
+    """Requests that fill row tiles of their own: prefixes that end at a key tile and beside one; tokens without own keys."""
+    rng = np.random.default_rng(dim + sum(counts))
+    for prefix in (1, 63, 64, 65, 300):
+        call = make(rng, counts, lengths, prefix, 8, 1, dim, 16, padding=2)
+        check_attention(hip_device, call)
+        call[6][prefix // 32] = -1  # a page of the prefix that is not there
+        check_attention(hip_device, call)
+
+
+def test_attention_offsets_that_do_not_ascend_leave_zeros(hip_device):
+    rng = np.random.default_rng(21)
+    call = make(rng, [3, 40, 1], [9, 50, 70], 30, 4, 1, 64, 16)
+    for offsets in ([0, 43, 3, 44], [0, 3, 43, 42], [0, 2 ** 31 - 1, -1, 44]):
+        call[3] = np.array(offsets, np.int32)
+        assert (run_attention(hip_device, *call) == 0).all()
+
+
 def test_attention_long_and_short_requests_share_a_call(hip_device):
     rng = np.random.default_rng(2)
     lengths = [4000, 1, 90, 700, 3, 1500]

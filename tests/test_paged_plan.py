@@ -29,12 +29,27 @@ struct Item { int list, b, head, tile; bool operator<(const Item& o) const {
 
 // 0, or the line that found a fault
 #define NEED(...) if (!(__VA_ARGS__)) return __LINE__
+int leads = 0;
+extern "C" int led() { return leads; }
 extern "C" int walk(int tokens, int requests, int heads, int kv, int shift, int columns, int prefix_columns, const int* offsets,
                     const int* lengths, int prefix_length, int monotone) {
   Extents e = extents(tokens, requests, heads, kv, shift, columns, prefix_columns);
-  auto request = [&](int b) {
-    return b == requests ? prefix_request(e, offsets[b], prefix_length) : own_request(e, offsets[b], offsets[b + 1], lengths[b]);
-  };
+  Request prefix = prefix_request(e, offsets[requests], prefix_length);
+  auto request = [&](int b) { return b == requests ? prefix : own_request(e, offsets[b], offsets[b + 1], lengths[b]); };
+  int64_t items = 0;
+  bool apart = false;
+  for (int b = 0; b < requests; ++b) {
+    const Request r = request(b);
+    apart |= r.count && (r.narrow || !r.keys);
+    items += head_items(e, r);
+  }
+  e.lead = apart || !monotone ? 0 : lead_tiles(e, prefix, (int)items);
+  if (e.lead) {
+    NEED(e.lead == (prefix.keys + kWideKeys - 1) / kWideKeys);
+    NEED((items - row_tiles(e, prefix)) * e.lead <= (int64_t)row_tiles(e, prefix) * kSlotCost);
+    prefix.count = prefix.keys = 0;
+    ++leads;
+  }
   int64_t tiles = 0;
   for (int b = 0; b <= requests; ++b) {
     const Request r = request(b);
@@ -92,7 +107,7 @@ extern "C" int walk(int tokens, int requests, int heads, int kv, int shift, int 
         const int sees = r.prefix ? r.keys : least(r.keys, most(0, r.behind + i + 1));
         const auto at = reached.find(Item{k, b, head, tile});
         if (r.keys == 0) { NEED(at == reached.end()); }
-        else NEED(at != reached.end() && (int64_t)at->second * (k ? kNarrowKeys : kWideKeys) >= sees);
+        else NEED(at != reached.end() && (int64_t)(at->second - (r.prefix ? 0 : e.lead)) * (k ? kNarrowKeys : kWideKeys) >= sees);
         const TokenSlots rows = token_slots(e, r, b, starts[k][b], r.first + i);
         const Slots s = rows.in(head, quota[k]);
         NEED(!rows.tiles || rows.row + share <= (k ? kNarrowRows : kWideRows));
@@ -154,6 +169,26 @@ def test_segments_cover_every_item_once(library, seed):
     heads, kv, shift, columns, prefix_columns, offsets, lengths, prefix = call(rng)
     tokens = offsets[-1] + rng.choice((0, 0, 5))
     assert walk(library, tokens, heads, kv, shift, columns, prefix_columns, offsets, lengths, prefix) == 0
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_prefix_leads_the_items_of_prompts(library, seed):
+    rng = random.Random(500 + seed)
+    heads, kv = rng.choice(((32, 8), (16, 16), (28, 4), (16, 1), (5, 5)))
+    requests = rng.choice((1, 2, 3, 17))
+    counts = [rng.choice((rng.randint(20, 90), 128, rng.randint(200, 600))) for _ in range(requests)]
+    if rng.random() < 0.3:
+        counts[rng.randrange(requests)] = 0
+        counts.append(40)
+    shift = rng.choice((0, 4, 6))
+    lengths = [n + rng.choice((0, 0, rng.randint(0, 3000))) for n in counts]
+    prefix = rng.choice((1, 63, 64, 65, rng.randint(100, 5000)))
+    offsets = [sum(counts[:b]) for b in range(len(counts) + 1)]
+    columns = -(-max(lengths) // (1 << shift))
+    before = library.led()
+    assert walk(library, offsets[-1], heads, kv, shift, columns, -(-prefix // (1 << shift)), offsets, lengths, prefix) == 0
+    if len(counts) == 1 and counts[0] * (heads // kv) > 16:
+        assert library.led() == before + 1
 
 
 @pytest.mark.parametrize("seed", range(40))
