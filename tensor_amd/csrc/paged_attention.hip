@@ -723,7 +723,8 @@ __device__ __forceinline__ int wave_scan(int v) {
 // A token's rows in the slots of one list, as the joining kernel reads them: half a record.
 struct TokenPart {
   TokenSlots at;
-  int quota, narrow;
+  Quota quota;
+  __device__ bool narrow() const { return quota.few >= 0; }
 };
 static_assert(sizeof(TokenPart) == 2 * kRecord, "a record is two parts");
 
@@ -799,7 +800,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
     starts[tid][lists] = tid ? done[1] : done[0];
   }
   __syncthreads();
-  const int quota[2] = {(done[0] + kGroups - 1) / kGroups, (done[1] + kStreams - 1) / kStreams};
+  const Quota wide = wide_quota(done[0]), narrow = narrow_quota(done[1], wide.many);
   const bool alone = all.keys == 0;
   float* const slots = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + record_bytes(a.tokens));
 
@@ -822,10 +823,10 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
   auto wide_list = [&]() {
     // Workgroups go round the eight XCDs in turn: neighbouring ranges, which read the same keys, are given to
     // one XCD, whose L2 then serves most of them.
-    const int ranges = quota[0] ? (done[0] + quota[0] - 1) / quota[0] : 0, share = (ranges + 7) / 8;
+    const int ranges = wide.many ? (done[0] + wide.many - 1) / wide.many : 0, share = (ranges + 7) / 8;
     const int range = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= share || range >= ranges) return;
-    Walk<decltype(requests)> walk(x, starts[0], requests, range * quota[0], min((range + 1) * quota[0], done[0]));
+    Walk<decltype(requests)> walk(x, starts[0], requests, range * wide.many, min((range + 1) * wide.many, done[0]));
     Segment seg;
     for (settle(walk); walk.next(seg); walk.advance(), settle(walk)) {
       wide_segment<D>(a, x, walk.r, seg, list_of(walk.r, walk.b), prefix_keys,
@@ -835,8 +836,10 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
   };
   auto narrow_list = [&]() {
     float* const base = slots + slot_floats(kWideRows, D) * (size_t)wide_slots(x);
-    const int stream = wave * kGroups + blockIdx.x;  // neighbours in the list run on different CUs
-    const int from = stream * quota[1], to = min(from + quota[1], done[1]);
+    // first the workgroups without wide work; neighbours in the list run on different CUs
+    constexpr int half = kGroups / 2;
+    const int stream = ((blockIdx.x < half) == (wide.many > 0) ? kStreams / 2 : 0) + wave * half + blockIdx.x % half;
+    const int from = narrow.begin(stream), to = min(narrow.begin(stream + 1), done[1]);
     if (from >= to) return;
     Walk<decltype(requests)> walk(x, starts[1], requests, from, to);
     Segment seg;
@@ -861,7 +864,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
       TokenPart to{};
       const int b = part ? own : a.requests;
       if (real)
-        to = TokenPart{token_slots(x, r, b, starts[r.narrow][b], t), r.narrow ? quota[1] : quota[0], r.narrow};
+        to = TokenPart{token_slots(x, r, b, starts[r.narrow][b], t), r.narrow ? narrow : wide};
       record[part] = to;
       r = all;
     }
@@ -890,10 +893,10 @@ __global__ __launch_bounds__(THREADS) void join_segments(const AttentionArgs a, 
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const Slots s = parts[k].at.in(kv_head, parts[k].quota);
-    const int rows = parts[k].narrow ? kNarrowRows : kWideRows, at = parts[k].at.row + j;
+    const int rows = parts[k].narrow() ? kNarrowRows : kWideRows, at = parts[k].at.row + j;
     count[k] = s.count;
     stride[k] = slot_floats(rows, D);
-    from[k] = slots + (parts[k].narrow ? slot_floats(kWideRows, D) * (size_t)wide_slots(x) : 0) + stride[k] * (size_t)s.first + at;
+    from[k] = slots + (parts[k].narrow() ? slot_floats(kWideRows, D) * (size_t)wide_slots(x) : 0) + stride[k] * (size_t)s.first + at;
     sum_at[k] = rows;
     out_at[k] = 2 * rows + at * (D - 1) + 4 * lane;
   }

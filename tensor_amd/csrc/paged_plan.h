@@ -4,8 +4,9 @@
 // The work is two lists of key tiles.  Item = the rows of one request (or of all tokens, against the shared
 // prefix) and one key head, in row tiles: wide ones of up to 128 rows against tiles of 64 keys, and
 // narrow ones of up to 16 rows (decode) against tiles of 32.  The wide list is cut into equal ranges, one for
-// each workgroup, the narrow list into equal ranges, one for each wave; a range crosses items, so the
-// work is even whatever the lengths.  The part of an item in one range is a segment; it leaves its
+// each workgroup, or, if it is short, for each of the first half; the narrow list is cut into ranges for waves, of
+// which those of the second half of the workgroups take more where the first has wide work.  A range crosses
+// items, so the work is even whatever the lengths.  The part of an item in one range is a segment; it leaves its
 // rows' maxima, sums and outputs in a slot of the workspace, and a second kernel joins the slots of a row.
 // Slot = item + range: both only grow along the list, one of them with every segment.  To begin a wide item
 // costs a workgroup as much as kItemCost tiles, so in long lists each has that many empty positions before its
@@ -32,10 +33,12 @@ constexpr int kGroups = 512;                // workgroups: two per CU
 constexpr int kStreams = kGroups * kWaves;  // waves of the launch
 constexpr int kWideRows = 128, kWideKeys = 64, kNarrowRows = 16, kNarrowKeys = 32;
 constexpr int kItemCost = 3, kLongRange = 24;  // tiles of a range from which items have a cost
+constexpr int kBeside = 300;                    // narrow tiles of half the workgroups beside each wide tile of a range
 constexpr int kSlotCost = 8;                   // to begin an item, leave its rows in a slot and join them, in tiles
 
 PAGED_CODE int least(int a, int b) { return a < b ? a : b; }
 PAGED_CODE int most(int a, int b) { return a > b ? a : b; }
+PAGED_CODE int64_t most64(int64_t a, int64_t b) { return a > b ? a : b; }
 
 // Extents of a call; rows of wide tiles are whole tokens.
 struct Extents {
@@ -233,8 +236,35 @@ struct Walk {
   }
 };
 
+// Positions of a list's ranges: `many` for each (few < 0), or for the first kStreams / 2 and `few` for the others.
+struct Quota {
+  int many, few;
+  PAGED_CODE int range(int at) const {
+    constexpr int half = kStreams / 2;
+    const int others = at - half * many;
+    const bool late = few >= 0 && others >= 0;
+    return (late ? others : at) / (late ? few : many) + (late ? half : 0);
+  }
+  PAGED_CODE int begin(int range) const {
+    constexpr int half = kStreams / 2;
+    return few < 0 || range <= half ? range * many : half * many + (range - half) * few;
+  }
+};
+// Short lists go to half the workgroups, one on a CU, which shares its bandwidth with one that has narrow work, and
+// leave half the slots.
+PAGED_CODE Quota wide_quota(int positions) {
+  const int ranges = positions < kLongRange * kGroups ? kGroups / 2 : kGroups;
+  return Quota{(positions + ranges - 1) / ranges, -1};
+}
+// `wide`: positions of a wide range.  While the first half of the workgroups have those, the others take kBeside
+// narrow tiles for each; the rest is for all.
+PAGED_CODE Quota narrow_quota(int positions, int wide) {
+  const int few = (int)(most64(positions - (int64_t)kBeside * wide, 0) / kStreams);
+  return Quota{(positions - few * (kStreams / 2) + kStreams / 2 - 1) / (kStreams / 2), few};
+}
+
 // The slots of a token's rows in request b's list, whose first position is `start`: `in` gives those of one
-// key head, in ranges of `quota` positions.
+// key head.
 struct Slots {
   int first, count;
 };
@@ -242,10 +272,10 @@ struct TokenSlots {
   int t0, tiles, span;  // position of the first key tile of the rows' item of key head 0, its tiles, positions of a head
   int item, items;      // that item, items of a head
   int row;              // the token's first row within a slot
-  PAGED_CODE Slots in(int head, int quota) const {
-    if (!tiles || !quota) return Slots{0, 0};
-    const int from = t0 + head * span, range = from / quota;
-    return Slots{item + head * items + range, (from + tiles - 1) / quota - range + 1};
+  PAGED_CODE Slots in(int head, const Quota& quota) const {
+    if (!tiles || !quota.many) return Slots{0, 0};
+    const int from = t0 + head * span, range = quota.range(from);
+    return Slots{item + head * items + range, quota.range(from + tiles - 1) - range + 1};
   }
 };
 PAGED_CODE TokenSlots token_slots(const Extents& e, const Request& r, int b, int start, int token) {

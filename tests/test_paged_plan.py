@@ -69,14 +69,16 @@ extern "C" int walk(int tokens, int requests, int heads, int kv, int shift, int 
   std::map<Item, std::vector<int64_t>> slots;  // slots of an item's segments, in order
   std::map<Item, int> reached;
   std::set<int64_t> used[2];
-  int quota[2];
+  Quota quota[2];
   for (int k = 0; k < 2; ++k) {
     starts[k].push_back(done[k]);
     const int ranges = k ? kStreams : kGroups;
-    quota[k] = (int)((done[k] + ranges - 1) / ranges);
+    quota[k] = k ? narrow_quota((int)done[1], quota[0].many) : wide_quota((int)done[0]);
+    NEED(quota[k].begin(ranges) >= done[k] && (quota[k].few >= 0) == (k == 1));
     for (int range = 0; range < ranges; ++range) {
-      const int64_t from = (int64_t)range * quota[k], to = from + quota[k] < done[k] ? from + quota[k] : done[k];
+      const int64_t from = quota[k].begin(range), to = least(quota[k].begin(range + 1), (int)done[k]);
       if (from >= to) continue;
+      NEED(quota[k].range((int)from) == range && quota[k].range((int)to - 1) == range);
       Walk<decltype(request)> walk(e, starts[k].data(), request, (int)from, (int)to);
       Segment s;
       int taken = 0;
@@ -95,7 +97,7 @@ extern "C" int walk(int tokens, int requests, int heads, int kv, int shift, int 
         NEED(s.all == (slots[item].size() == 1 && s.t1 == item_tiles(e, r, s.tile)));
         taken += s.t1 - s.t0;
       }
-      NEED(taken <= quota[k]);
+      NEED(taken <= to - from);
     }
   }
   for (int b = 0; b <= requests; ++b) {
