@@ -57,12 +57,15 @@ __device__ __forceinline__ half8_t join(half4_t a, half4_t b) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// The 16-byte chunk at which a row of a staged tile keeps chunk c: fragment reads of keys take one
-// chunk of eight consecutive rows at a time, transposed reads of values two chunks of four rows.
+// The 16-byte chunk at which a row of a staged tile keeps chunk c, so that the lanes of half a wave read 64 different
+// banks: keys' fragments are one chunk of eight consecutive rows, values' transposed ones four chunks of four rows
+// (wide) or two of eight (narrow).
 template <int D>
 __device__ __forceinline__ int key_chunk(int row, int c) { return c ^ (row & (D / 8 - 1)); }
 template <int D>
-__device__ __forceinline__ int value_chunk(int row, int c) { return c ^ (2 * (row & (D / 16 - 1))); }
+__device__ __forceinline__ int wide_value_chunk(int row, int c) { return c ^ (4 * (D == 128 ? row & 3 : (row >> 1) & 1)); }
+template <int D>
+__device__ __forceinline__ int narrow_value_chunk(int row, int c) { return c ^ (2 * (row & (D / 16 - 1))); }
 
 // Loads of these values are waited for here, where no tile is on its way: the compiler, which does not know
 // of those, waits for all loads before a value's first use.
@@ -308,7 +311,7 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
   for (int n = 0; n < N; ++n) {
     const int kr = r0 + n * RPI + lane / CH;
     k_lane[n] = 2 * ((lane / CH) * D + 8 * key_chunk<D>(kr, lane % CH));
-    v_lane[n] = 2 * ((lane / CH) * D + 8 * value_chunk<D>(kr, lane % CH));
+    v_lane[n] = 2 * ((lane / CH) * D + 8 * wide_value_chunk<D>(kr, lane % CH));
   }
   float16_t o[DB] = {};
   float m = -kInfinity, l = 0.0f, top;
@@ -326,7 +329,7 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
     for (int db = 0; db < DB; ++db) {
       const int vr = 4 * half + ((lane & 15) >> 2);
       v_at[db] = lds_at + 4 * MAT +
-                 2 * (vr * D + 8 * value_chunk<D>(vr, 4 * db + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 4 * (lane & 1));
+                 2 * (vr * D + 8 * wide_value_chunk<D>(vr, 4 * db + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 4 * (lane & 1));
     }
   };
   // S^T = K Q^T of 32 keys, `between(n)` after each of its D / 16 products; fragment reads stay AHEAD of them
@@ -578,7 +581,7 @@ __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Ext
   for (int n = 0; n < PER; ++n) {
     const int kr = n * RPI + lane / CH;
     k_lane[n] = 2 * ((lane / CH) * D + 8 * key_chunk<D>(kr, lane % CH));
-    v_lane[n] = 2 * ((lane / CH) * D + 8 * value_chunk<D>(kr, lane % CH));
+    v_lane[n] = 2 * ((lane / CH) * D + 8 * narrow_value_chunk<D>(kr, lane % CH));
   }
   float4_t o[DB] = {};
   float m = -kInfinity, l = 0.0f;
@@ -664,7 +667,7 @@ __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Ext
     half8_t v[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
-      const int vr = 4 * quad + (row >> 2), chunk = value_chunk<D>(vr, 2 * db + ((lane & 3) >> 1));
+      const int vr = 4 * quad + (row >> 2), chunk = narrow_value_chunk<D>(vr, 2 * db + ((lane & 3) >> 1));
       const uint32_t at = lds_at + 2 * (MAT + vr * D + 8 * chunk + 4 * (lane & 1));
       v[db] = join(read_transposed(at), read_transposed(at + 32 * D));
     }
