@@ -448,11 +448,6 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
     auto load_v = [&](int t, const Tile& of) { of.load(keys, t * kWideKeys, r0, keys.v, v_lane, place_at(t) + 4 * MAT); };
     auto step = [&](int t, auto more1, auto more2) {  // of tiles t + 1 and t + 2
       constexpr bool MORE1 = decltype(more1)::value, MORE2 = decltype(more2)::value;
-      // of the two workgroups of a CU the older one's waves go first: the younger's take their turn every other tile
-      if (blockIdx.x >= kGroups / 2) {
-        if (t & 1) __builtin_amdgcn_s_setprio(1);
-        else __builtin_amdgcn_s_setprio(0);
-      }
       // V(t) has landed (K(t + 1) may be on its way), this wave's rows and after the barrier everyone's;
       // nobody reads V(t - 1) any more
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MORE1 ? N : 0) : "memory");
@@ -515,7 +510,6 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
       ++t;
     }
     step(t, std::false_type{}, std::false_type{});
-    __builtin_amdgcn_s_setprio(0);
     if (__syncthreads_or(odd)) {
       for (int key = max(t0, max(safe, 0) / kWideKeys) * kWideKeys; key < min(t1 * kWideKeys, bound); ++key) {
         const int page = keys.entry(key >> x.page_shift);
@@ -793,7 +787,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
     done[1] += all.narrow ? span : 0;
     done[2] += a.kv * head_items(x, all);
   }
-  x.cost = item_cost(done[0]);
+  x.cost = item_cost(done[2]);
   if (x.cost + x.lead)  // each thread its own entries
     for (int b = tid; b < a.requests; b += kThreads) starts[0][b] += (x.cost + x.lead) * starts[2][b];
   done[0] += x.cost * done[2];
@@ -803,7 +797,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
     starts[tid][lists] = tid ? done[1] : done[0];
   }
   __syncthreads();
-  const Quota wide = wide_quota(done[0]), narrow = narrow_quota(done[1], wide.many);
+  const Quota wide = wide_quota(done[0], done[1]), narrow = narrow_quota(done[1], wide.many);
   const bool alone = all.keys == 0;
   float* const slots = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + record_bytes(a.tokens));
 

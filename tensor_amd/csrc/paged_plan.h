@@ -146,7 +146,7 @@ PAGED_CODE int head_span(const Extents& e, const Request& r) {
 }
 // Items of one key head in the wide list.
 PAGED_CODE int head_items(const Extents& e, const Request& r) { return r.count && r.keys && !r.narrow ? row_tiles(e, r) : 0; }
-PAGED_CODE int item_cost(int tiles) { return tiles >= kLongRange * kGroups ? kItemCost : 0; }  // by the wide list's tiles
+PAGED_CODE int item_cost(int items) { return items >= kGroups / 4 ? kItemCost : 0; }  // by the wide list's items
 // Key tiles of a row tile.
 PAGED_CODE int item_tiles(const Extents& e, const Request& r, int tile) {
   if (r.narrow) return (r.keys + kNarrowKeys - 1) / kNarrowKeys;
@@ -252,8 +252,8 @@ struct Quota {
 };
 // Short lists go to half the workgroups, one on a CU, which shares its bandwidth with one that has narrow work, and
 // leave half the slots.
-PAGED_CODE Quota wide_quota(int positions) {
-  const int ranges = positions < kLongRange * kGroups ? kGroups / 2 : kGroups;
+PAGED_CODE Quota wide_quota(int positions, int narrow) {
+  const int ranges = narrow && positions < kLongRange * kGroups ? kGroups / 2 : kGroups;
   return Quota{(positions + ranges - 1) / ranges, -1};
 }
 // `wide`: positions of a wide range.  While the first half of the workgroups have those, the others take kBeside

@@ -50,12 +50,9 @@ extern "C" int walk(int tokens, int requests, int heads, int kv, int shift, int 
     prefix.count = prefix.keys = 0;
     ++leads;
   }
-  int64_t tiles = 0;
-  for (int b = 0; b <= requests; ++b) {
-    const Request r = request(b);
-    if (!r.narrow) tiles += (int64_t)kv * head_span(e, r);
-  }
-  e.cost = item_cost((int)tiles);
+  int64_t all = 0;
+  for (int b = 0; b <= requests; ++b) all += (int64_t)kv * head_items(e, request(b));
+  e.cost = item_cost((int)all);
   std::vector<int32_t> starts[2];
   int64_t done[2] = {0, 0};
   for (int b = 0; b <= requests; ++b) {
@@ -73,7 +70,7 @@ extern "C" int walk(int tokens, int requests, int heads, int kv, int shift, int 
   for (int k = 0; k < 2; ++k) {
     starts[k].push_back(done[k]);
     const int ranges = k ? kStreams : kGroups;
-    quota[k] = k ? narrow_quota((int)done[1], quota[0].many) : wide_quota((int)done[0]);
+    quota[k] = k ? narrow_quota((int)done[1], quota[0].many) : wide_quota((int)done[0], (int)done[1]);
     NEED(quota[k].begin(ranges) >= done[k] && (quota[k].few >= 0) == (k == 1));
     for (int range = 0; range < ranges; ++range) {
       const int64_t from = quota[k].begin(range), to = least(quota[k].begin(range + 1), (int)done[k]);
