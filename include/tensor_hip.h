@@ -328,10 +328,10 @@ int32_t tensor_rotary_store_v1(const TensorCallV1 *call, TensorErrorV1 *error);
  * Attention of every request's new tokens (the last counts of its lengths) over the shared prefix and its
  * own pages, causal within them: out[t, h] = sum_j softmax_j(scale q[t, h] . k[j]) v[j] over the prefix's
  * keys and the own keys up to the token's place.  Query head h reads key head h / (heads / kv_heads).  One
- * token or many for each request, in any mix.  The prefix is read once for the whole batch.  Scores, sums
- * and outputs are kept in fp32; the softmax weights enter the second product as fp16.  A token that sees
+ * token or many for each request, in any mix.  The prefix is read for 128 rows at a time, of whatever requests,
+ * not for each request.  Scores, sums and outputs are kept in fp32; the softmax weights enter the second product as fp16.  A token that sees
  * no key gives zeros, and so does a row of q past the last request.  A table entry that is no page of the
- * cache hides its keys.
+ * cache hides its keys; offsets that do not ascend leave every row zeros.
  *    0 q             fp16 [T, heads, dim], dim 64 or 128
  *    1 k_cache, 2 v_cache  fp16 [pages, kv_heads, page_size, dim]
  *    3 offsets       int32 [B + 1]  first row of each request's tokens (B up to 1024)

@@ -8,13 +8,19 @@
 // which those of the second half of the workgroups take more where the first has wide work.  A range crosses
 // items, so the work is even whatever the lengths.  The part of an item in one range is a segment; it leaves its
 // rows' maxima, sums and outputs in a slot of the workspace, and a second kernel joins the slots of a row.
-// Slot = item + range: both only grow along the list, one of them with every segment.  To begin a wide item
-// costs a workgroup as much as kItemCost tiles, so in long lists each has that many empty positions before its
-// first tile (in short ones a range of one more tile would cost more than it evens out).
+// Slot = item + range: both only grow along the list, one of them with every segment.
+//
+// Narrow tiles waste the matrix cores, wide ones the loads of rows that are not there: 16 rows are level (16 requests of 4
+// tokens and 4 heads a key head, 16000 keys: 208 us narrow, 204 wide; 1000 keys: 66 and 65), and fewer stay narrow.
+//
+// To begin a wide item costs a workgroup as much as kItemCost tiles, so where there is an item for every fourth
+// workgroup each has that many empty positions before its first tile (a prompt of 1024 tokens: 45 us, 56 without; 16
+// requests of 33 tokens behind 8192 keys: 123 and 156; but 64 requests behind 16384 keys, 16 items: 62 and 59).
 //
 // The prefix is a list entry of its own where tokens of several requests fill its row tiles; where each request
 // fills tiles of its own (prompts, one request), its wide items begin with the prefix's tiles instead (`lead`),
-// which leaves one slot less to write and join.
+// which leaves one slot less to write and join (3 requests of 1024 tokens behind 8192 keys: 422 us, 447 apart; 8 of 128
+// behind 4096: 114 and 129; but 16 of 33 behind 8192, whose tiles would be half empty: 173, and 121 apart).
 #pragma once
 
 #include <stddef.h>
@@ -32,9 +38,10 @@ constexpr int kWaves = 4;                   // of a workgroup
 constexpr int kGroups = 512;                // workgroups: two per CU
 constexpr int kStreams = kGroups * kWaves;  // waves of the launch
 constexpr int kWideRows = 128, kWideKeys = 64, kNarrowRows = 16, kNarrowKeys = 32;
-constexpr int kItemCost = 3, kLongRange = 24;  // tiles of a range from which items have a cost
-constexpr int kBeside = 300;                    // narrow tiles of half the workgroups beside each wide tile of a range
-constexpr int kSlotCost = 8;                   // to begin an item, leave its rows in a slot and join them, in tiles
+constexpr int kItemCost = 3;                // to begin an item, in tiles
+constexpr int kSlotCost = 8;                // that, and to leave its rows in a slot and join them
+constexpr int kLongRange = 24;              // tiles of a range from which a wide list is long
+constexpr int kBeside = 300;                // narrow tiles of half the workgroups beside each wide tile of a range
 
 PAGED_CODE int least(int a, int b) { return a < b ? a : b; }
 PAGED_CODE int most(int a, int b) { return a > b ? a : b; }
@@ -45,7 +52,7 @@ struct Extents {
   int tokens, requests, kv, share, page_shift, columns, prefix_columns;  // share: query heads of a key head
   int per;                                                               // tokens of a wide row tile
   int cost;                                                              // positions before a wide item's first tile
-  int lead;                                                              // tiles of the prefix, of which its requests' items consist first
+  int lead;                                                              // tiles of the prefix that begin each of them
 };
 PAGED_CODE Extents extents(int tokens, int requests, int heads, int kv, int page_shift, int columns, int prefix_columns) {
   const int share = heads / kv;
@@ -250,14 +257,16 @@ struct Quota {
     return few < 0 || range <= half ? range * many : half * many + (range - half) * few;
   }
 };
-// Short lists go to half the workgroups, one on a CU, which shares its bandwidth with one that has narrow work, and
-// leave half the slots.
+// A short list beside a narrow one goes to half the workgroups, one on a CU, whose other one reads the narrow list's
+// keys meanwhile, and leaves half the slots (64 requests behind 16384 keys: 59 us, 72 with all; 12 requests of 5 tokens:
+// 29.6 and 33.7).  A long one needs all (3 x 1024 tokens: 425 us, 499 with half), and so does one alone (a prompt of
+// 1024 tokens: 56 us, 63 with half).
 PAGED_CODE Quota wide_quota(int positions, int narrow) {
   const int ranges = narrow && positions < kLongRange * kGroups ? kGroups / 2 : kGroups;
   return Quota{(positions + ranges - 1) / ranges, -1};
 }
 // `wide`: positions of a wide range.  While the first half of the workgroups have those, the others take kBeside
-// narrow tiles for each; the rest is for all.
+// narrow tiles for each; the rest is for all (64 requests behind 16384 keys: 57 us, 65 in equal shares).
 PAGED_CODE Quota narrow_quota(int positions, int wide) {
   const int few = (int)(most64(positions - (int64_t)kBeside * wide, 0) / kStreams);
   return Quota{(positions - few * (kStreams / 2) + kStreams / 2 - 1) / (kStreams / 2), few};

