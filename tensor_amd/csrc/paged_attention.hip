@@ -38,6 +38,9 @@ typedef float float16_t __attribute__((ext_vector_type(16)));
 constexpr int kThreads = 64 * kWaves;
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ size_t uniform(size_t v) {
+  return (size_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v);
+}
 
 // threadIdx.x as a value of its own: what a segment derives from it is then not kept in registers outside
 __device__ __forceinline__ int here() {
@@ -225,7 +228,7 @@ struct Rows {
     if (fast) {
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g)
-        dma_rows<D>(reinterpret_cast<const uint8_t*>(matrix) + at[g], lane_at, dst + 32 * g * D);
+        dma_rows<D>(reinterpret_cast<const uint8_t*>(matrix) + uniform(at[g]), lane_at, dst + 32 * g * D);
     } else {
       int page[GROUPS * PER];
 #pragma unroll
@@ -766,8 +769,8 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
     const int b = base + tid;
     const bool real = b < a.requests;
     const Request r = request_of(a, x, min(b, a.requests - 1));
-    const int span = real ? a.kv * head_span(x, r) : 0;
-    const int mine[3] = {r.narrow ? 0 : span, r.narrow ? span : 0, real ? a.kv * head_items(x, r) : 0};
+    const int span = real ? head_span(x, r) : 0;
+    const int mine[3] = {r.narrow ? 0 : span, r.narrow ? span : 0, real ? head_items(x, r) : 0};
     const bool odd[2] = {(bool)__any(real && r.count && (r.narrow || !r.keys)), (bool)__any(real && a.offsets[b] > a.offsets[b + 1])};
     int scan[3];
 #pragma unroll
@@ -798,17 +801,17 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
 #pragma unroll
   for (int k = 0; k < 3; ++k) done[k] = uniform(done[k]);
   const int prefix_keys = uniform(all.keys);
-  x.lead = uniform(apart ? 0 : lead_tiles(x, all, done[2] / a.kv));
+  x.lead = uniform(apart ? 0 : lead_tiles(x, all, done[2]));
   if (x.lead) all.count = all.keys = 0;  // each request's items take it
   done[0] += x.lead * done[2];
   const int last[2] = {done[0], done[1]}, last_items = done[2];  // where the prefix begins
   {
-    const int span = a.kv * head_span(x, all);
+    const int span = head_span(x, all);
     done[0] += all.narrow ? 0 : span;
     done[1] += all.narrow ? span : 0;
-    done[2] += a.kv * head_items(x, all);
+    done[2] += head_items(x, all);
   }
-  x.cost = item_cost(done[2]);
+  x.cost = item_cost(a.kv * done[2]);
   if (x.cost + x.lead)  // each thread its own entries
     for (int b = tid; b < a.requests; b += kThreads) starts[0][b] += (x.cost + x.lead) * starts[2][b];
   done[0] += x.cost * done[2];
@@ -818,7 +821,8 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
     starts[tid][lists] = tid ? done[1] : done[0];
   }
   __syncthreads();
-  const Quota wide = wide_quota(done[0], done[1]), narrow = narrow_quota(done[1], wide.many);
+  const int positions[2] = {a.kv * done[0], a.kv * done[1]};
+  const Quota wide = wide_quota(positions[0], positions[1]), narrow = narrow_quota(positions[1], wide.many);
   const bool alone = all.keys == 0;
   float* const slots = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + record_bytes(a.tokens));
 
@@ -841,10 +845,10 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
   auto wide_list = [&]() {
     // Workgroups go round the eight XCDs in turn: neighbouring ranges, which read the same keys, are given to
     // one XCD, whose L2 then serves most of them.
-    const int ranges = wide.many ? (done[0] + wide.many - 1) / wide.many : 0, share = (ranges + 7) / 8;
+    const int ranges = wide.many ? (positions[0] + wide.many - 1) / wide.many : 0, share = (ranges + 7) / 8;
     const int range = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= share || range >= ranges) return;
-    Walk<decltype(requests)> walk(x, starts[0], requests, range * wide.many, min((range + 1) * wide.many, done[0]));
+    Walk<decltype(requests)> walk(x, starts[0], requests, wide_items(x), range * wide.many, min((range + 1) * wide.many, positions[0]));
     Segment seg;
     for (settle(walk); walk.next(seg); walk.advance(), settle(walk)) {
       wide_segment<D>(a, x, walk.r, seg, list_of(walk.r, walk.b), prefix_keys,
@@ -857,9 +861,9 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
     // first the workgroups without wide work; neighbours in the list run on different CUs
     constexpr int half = kGroups / 2;
     const int stream = ((blockIdx.x < half) == (wide.many > 0) ? kStreams / 2 : 0) + wave * half + blockIdx.x % half;
-    const int from = narrow.begin(stream), to = min(narrow.begin(stream + 1), done[1]);
+    const int from = narrow.begin(stream), to = min(narrow.begin(stream + 1), positions[1]);
     if (from >= to) return;
-    Walk<decltype(requests)> walk(x, starts[1], requests, from, to);
+    Walk<decltype(requests)> walk(x, starts[1], requests, narrow_items(x), from, to);
     Segment seg;
     for (settle(walk); walk.next(seg); walk.advance(), settle(walk)) {
       narrow_segment<D>(a, x, walk.r, seg, list_of(walk.r, walk.b),
@@ -882,7 +886,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
       TokenPart to{};
       const int b = part ? own : a.requests;
       if (real)
-        to = TokenPart{token_slots(x, r, b, starts[r.narrow][b], t), r.narrow ? narrow : wide};
+        to = TokenPart{token_slots(x, r, b, starts[r.narrow], r.narrow ? narrow_items(x) : wide_items(x), t), r.narrow ? narrow : wide};
       record[part] = to;
       r = all;
     }

@@ -6,7 +6,8 @@
 // narrow ones of up to 16 rows (decode) against tiles of 32.  The wide list is cut into equal ranges, one for
 // each workgroup, or, if it is short, for each of the first half; the narrow list is cut into ranges for waves, of
 // which those of the second half of the workgroups take more where the first has wide work.  A range crosses
-// items, so the work is even whatever the lengths.  The part of an item in one range is a segment; it leaves its
+// items, so the work is even whatever the lengths.  A list goes through all requests for one key head before the
+// next: workgroups of one XCD, which have neighbouring ranges, then read the same prefix.  The part of an item in one range is a segment; it leaves its
 // rows' maxima, sums and outputs in a slot of the workspace, and a second kernel joins the slots of a row.
 // Slot = item + range: both only grow along the list, one of them with every segment.
 //
@@ -63,10 +64,13 @@ PAGED_CODE Extents extents(int tokens, int requests, int heads, int kv, int page
 constexpr int kRecord = 16;  // 32-bit words
 PAGED_CODE size_t record_bytes(int tokens) { return ((size_t)tokens * 4 * kRecord + 255) / 256 * 256; }
 PAGED_CODE size_t slot_floats(int rows, int dim) { return (size_t)rows * (dim + 2); }
-PAGED_CODE int64_t wide_slots(const Extents& e) {
-  return (int64_t)e.kv * (e.tokens / e.per + e.requests + (e.tokens + e.per - 1) / e.per) + kGroups;
+// numbers of one key head's items
+PAGED_CODE int narrow_items(const Extents& e) { return e.requests + 1; }
+PAGED_CODE int wide_items(const Extents& e) {
+  return e.tokens / e.per + e.requests + (e.tokens + e.per - 1) / e.per;
 }
-PAGED_CODE int64_t narrow_slots(const Extents& e) { return (int64_t)e.kv * (e.requests + 1) + kStreams; }
+PAGED_CODE int64_t wide_slots(const Extents& e) { return (int64_t)e.kv * wide_items(e) + kGroups; }
+PAGED_CODE int64_t narrow_slots(const Extents& e) { return (int64_t)e.kv * narrow_items(e) + kStreams; }
 
 // sum over i < n of floor((a i + b) / m), by the Euclidean algorithm
 PAGED_CODE unsigned floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
@@ -167,11 +171,10 @@ PAGED_CODE int lead_tiles(const Extents& e, const Request& prefix, int items) {
   return !prefix.narrow && (int64_t)(items - own) * tiles <= (int64_t)own * kSlotCost ? tiles : 0;
 }
 
-// Items of request b (b = requests: the prefix) grow along the list and stay within the slots.
-PAGED_CODE int wide_item(const Extents& e, const Request& r, int b, int head, int tile) {
-  return e.kv * ((r.prefix ? r.count : r.first) / e.per + b) + head * row_tiles(e, r) + tile;
+// Number of an item among its key head's (b = requests: the prefix's): grows along the list.
+PAGED_CODE int item_number(const Extents& e, const Request& r, int b, int tile) {
+  return r.narrow ? b : (r.first + (r.prefix ? r.count : 0)) / e.per + b + tile;  // (the prefix's first is 0)
 }
-PAGED_CODE int narrow_item(const Extents& e, int b, int head) { return e.kv * b + head; }
 
 // largest i < count with start[i] <= t; start[0] <= t < start[count]
 PAGED_CODE int find(const int32_t* start, int count, int t) {
@@ -183,7 +186,8 @@ PAGED_CODE int find(const int32_t* start, int count, int t) {
   return lo;
 }
 
-// A range's way through its list: `requests(b)` gives request b, `start` the first position of each.
+// A range's way through its list: `requests(b)` gives request b, `start` the first position of each within a key
+// head and (the last) the head's positions, `items` the numbers of a head's items.
 struct Segment {
   int head, tile, t0, t1;  // key head, row tile, key tiles
   int item;
@@ -194,18 +198,17 @@ struct Walk {
   const Extents& e;
   const int32_t* start;
   const Requests& requests;
+  const int items;
   int left;             // positions of the range that are left
-  int b, head, tile;    // the item, and the position within it
-  int at;
+  int head, at, b;      // the item, and the position within it
+  int tile;
   Request r;
 
   // the range [from, to) of the list, from < to
-  PAGED_CODE Walk(const Extents& e, const int32_t* start, const Requests& requests, int from, int to)
-      : e(e), start(start), requests(requests), left(to - from), b(find(start, e.requests + 1, from)), r(requests(b)) {
-    const int span = (start[b + 1] - start[b]) / e.kv;
-    at = from - start[b];
-    head = at / span;
-    at -= head * span;
+  PAGED_CODE Walk(const Extents& e, const int32_t* start, const Requests& requests, int items, int from, int to)
+      : e(e), start(start), requests(requests), items(items), left(to - from), head(from / start[e.requests + 1]),
+        at(from - head * start[e.requests + 1]), b(find(start, e.requests + 1, at)), r(requests(b)) {
+    at -= start[b];
     tile = 0;
     if (!r.narrow) {
       int hi = row_tiles(e, r);  // the last row tile that begins at or before the position
@@ -225,7 +228,7 @@ struct Walk {
     s.tile = tile;
     s.t0 = at + skip - cost;
     s.t1 = least(tiles, s.t0 + left - skip);
-    s.item = r.narrow ? narrow_item(e, b, head) : wide_item(e, r, b, head, tile);
+    s.item = head * items + item_number(e, r, b, tile);
     s.all = s.t0 == 0 && s.t1 == tiles;
     left -= skip + s.t1 - s.t0;
     return true;
@@ -236,9 +239,9 @@ struct Walk {
     at = 0;
     if (++tile < (r.narrow ? 1 : row_tiles(e, r))) return;
     tile = 0;
-    if (++head < e.kv) return;
-    head = 0;
-    b = find(start, e.requests + 1, start[b + 1]);
+    const bool last = start[b + 1] == start[e.requests + 1];
+    head += last;
+    b = find(start, e.requests + 1, last ? 0 : start[b + 1]);
     r = requests(b);
   }
 };
@@ -272,8 +275,7 @@ PAGED_CODE Quota narrow_quota(int positions, int wide) {
   return Quota{(positions - few * (kStreams / 2) + kStreams / 2 - 1) / (kStreams / 2), few};
 }
 
-// The slots of a token's rows in request b's list, whose first position is `start`: `in` gives those of one
-// key head.
+// The slots of a token's rows in request b's list (`start` and `items` as above): `in` gives those of one key head.
 struct Slots {
   int first, count;
 };
@@ -287,17 +289,15 @@ struct TokenSlots {
     return Slots{item + head * items + range, quota.range(from + tiles - 1) - range + 1};
   }
 };
-PAGED_CODE TokenSlots token_slots(const Extents& e, const Request& r, int b, int start, int token) {
-  TokenSlots s{start, 0, 0, narrow_item(e, b, 0), 1, 0};
+PAGED_CODE TokenSlots token_slots(const Extents& e, const Request& r, int b, const int32_t* start, int items,
+                                  int token) {
+  TokenSlots s{start[b], 0, start[e.requests + 1], 0, 0, 0};
   if (!r.count || !r.keys) return s;
   const int i = token - r.first, tile = r.narrow ? 0 : i / e.per;
   s.tiles = item_tiles(e, r, tile);
-  s.span = head_span(e, r);
-  if (!r.narrow) {
-    s.t0 += wide_begin(e, r, tile) + e.cost;
-    s.item = wide_item(e, r, b, 0, tile);
-    s.items = row_tiles(e, r);
-  }
+  s.item = item_number(e, r, b, tile);
+  s.items = items;
+  if (!r.narrow) s.t0 += wide_begin(e, r, tile) + e.cost;
   s.row = (i - (r.narrow ? 0 : tile * e.per)) * e.share;
   return s;
 }

@@ -60,23 +60,24 @@ extern "C" int walk(int tokens, int requests, int heads, int kv, int shift, int 
     NEED(r.first >= 0 && r.count >= 0 && r.first + r.count <= tokens);
     NEED(r.keys >= 0 && r.keys <= (int64_t)(r.prefix ? prefix_columns : columns) << shift);
     for (int k = 0; k < 2; ++k) starts[k].push_back(done[k]);
-    done[r.narrow] += (int64_t)kv * head_span(e, r);
+    done[r.narrow] += head_span(e, r);
   }
-  NEED(done[0] + done[1] + 2 * kStreams <= most_tiles(e) && most_tiles(e) < (int64_t)1 << 31);
+  NEED(kv * (done[0] + done[1]) + 2 * kStreams <= most_tiles(e) && most_tiles(e) < (int64_t)1 << 31);
   std::map<Item, std::vector<int64_t>> slots;  // slots of an item's segments, in order
   std::map<Item, int> reached;
   std::set<int64_t> used[2];
   Quota quota[2];
   for (int k = 0; k < 2; ++k) {
     starts[k].push_back(done[k]);
+    done[k] *= kv;
     const int ranges = k ? kStreams : kGroups;
-    quota[k] = k ? narrow_quota((int)done[1], quota[0].many) : wide_quota((int)done[0], (int)done[1]);
+    quota[k] = k ? narrow_quota((int)done[1], quota[0].many) : wide_quota((int)done[0], (int)done[1] * kv);
     NEED(quota[k].begin(ranges) >= done[k] && (quota[k].few >= 0) == (k == 1));
     for (int range = 0; range < ranges; ++range) {
       const int64_t from = quota[k].begin(range), to = least(quota[k].begin(range + 1), (int)done[k]);
       if (from >= to) continue;
       NEED(quota[k].range((int)from) == range && quota[k].range((int)to - 1) == range);
-      Walk<decltype(request)> walk(e, starts[k].data(), request, (int)from, (int)to);
+      Walk<decltype(request)> walk(e, starts[k].data(), request, k ? narrow_items(e) : wide_items(e), (int)from, (int)to);
       Segment s;
       int taken = 0;
       for (; walk.next(s); walk.advance()) {
@@ -107,7 +108,7 @@ extern "C" int walk(int tokens, int requests, int heads, int kv, int shift, int 
         const auto at = reached.find(Item{k, b, head, tile});
         if (r.keys == 0) { NEED(at == reached.end()); }
         else NEED(at != reached.end() && (int64_t)(at->second - (r.prefix ? 0 : e.lead)) * (k ? kNarrowKeys : kWideKeys) >= sees);
-        const TokenSlots rows = token_slots(e, r, b, starts[k][b], r.first + i);
+        const TokenSlots rows = token_slots(e, r, b, starts[k].data(), k ? narrow_items(e) : wide_items(e), r.first + i);
         const Slots s = rows.in(head, quota[k]);
         NEED(!rows.tiles || rows.row + share <= (k ? kNarrowRows : kWideRows));
         const auto& wrote = slots[Item{k, b, head, tile}];
