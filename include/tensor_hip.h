@@ -294,7 +294,8 @@ int32_t tensor_gguf_dequant_v1(const TensorCallV1 *call, TensorErrorV1 *error);
  *    7 offsets     int32 [B + 1] out: first row of each request's tokens, then their number
  *    8 lengths_out int32 [B]     out: lengths + counts
  *    9 positions   int32 [T]     out: start + place in the request; -1 past the last token
- *   10 slots       int32 [T]     out: slot; -1 past the last token and for a token without a page
+ *   10 slots       int32 [T]     out: slot; -1 past the last token, for a token without a page and for a
+ *                                 page whose slots pass int32
  *   11 table_out   int32 [B, P]  out: the table with the new pages
  *   12 free_left   int32 [1]     out: free_count less the pages taken; negative: so many were missing,
  *                                 and the entries that lack one are -1

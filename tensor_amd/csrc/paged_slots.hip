@@ -63,7 +63,8 @@ __global__ __launch_bounds__(kThreads) void paged_slots(const SlotsArgs a) {
   for (int64_t i = first; i < room; i += stride) {
     const int64_t place = l + i, column = place >> a.page_shift;
     const int32_t p = column < a.columns ? page((int)column) : -1;
-    a.slots[tokens + i] = p < 0 ? -1 : (p << a.page_shift) + (int)(place & (S - 1));
+    // (a page whose slots pass 31 bits has none: a wrapped one would be another page's)
+    a.slots[tokens + i] = p < 0 || p >> (31 - a.page_shift) ? -1 : (p << a.page_shift) + (int)(place & (S - 1));
     a.positions[tokens + i] = (int)(start + place);
   }
   if (blockIdx.y == 0 && tid == 0) {

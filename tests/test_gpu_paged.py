@@ -82,6 +82,17 @@ def test_slots_edges(hip_device):
     check_slots(hip_device, [6, 1], [1, 1], 0, [90], 1, np.array([[3, -1, -1, -1], [-1, -1, -1, -1]]), 2, 4)
 
 
+def test_slots_of_pages_past_int32(hip_device):
+    """A page whose slots int32 does not hold gives none, not those of another page; the last that fits has its own."""
+    page = 1024
+    fits, wraps = (1 << 21) - 1, (1 << 22) + 1  # the latter's slots would wrap to page 1's
+    table = np.array([[fits, -1], [wraps, -1], [1 << 21, -1]])
+    _, _, positions, slots, out, left = run_slots(hip_device, [1023, 5, 0], [2, 1, 1], 0, [wraps, 1 << 21], 2, table, 4, page)
+    assert slots.tolist() == [2 ** 31 - 1, -1, -1, -1]
+    assert positions.tolist() == [1023, 1024, 5, 0]
+    assert out.tolist() == [[fits, 1 << 21], [wraps, -1], [wraps, -1]] and left.tolist() == [0]
+
+
 def test_slots_share_a_long_prompt_and_a_wide_table(hip_device):
     rng = np.random.default_rng(5)
     table = rng.integers(0, 1 << 20, (3, 9001))
