@@ -14,9 +14,9 @@
 // Decode is bound by the cache's bytes: 256 requests of up to 4096 keys (2.1 GB, 8 key heads of 128) take 0.40 ms,
 // 5.3 TB/s, where a copy of 2 GiB moves 5.0; one request behind a prefix of 131071 keys (0.54 GB) takes 107 us, 5.0
 // TB/s.  Prompts are bound by the matrix cores and the power they draw (the clock falls to 1.6 GHz): 3 requests of 1024
-// tokens behind 8192 + 1024 keys (325 GFLOP) take 0.41 ms, 0.79 PFLOP/s, 35 us of it joining, where an fp16 product of
+// tokens behind 8192 + 1024 keys (325 GFLOP) take 0.39 ms, 0.83 PFLOP/s, 30 us of it joining, where an fp16 product of
 // 8192^3 reaches 1.16.  The smallest calls are two launches and their chains of loads: one token of 1021 keys takes
-// 12.6 us, 7 and 5.5 us of it the kernels.
+// 12.4 us, 7 and 5.5 us of it the kernels.
 #include <type_traits>
 
 #include "gguf_common.h"

@@ -7,8 +7,10 @@
 // each workgroup, or, if it is short, for each of the first half; the narrow list is cut into ranges for waves, of
 // which those of the second half of the workgroups take more where the first has wide work.  A range crosses
 // items, so the work is even whatever the lengths.  A list goes through all requests for one key head before the
-// next: workgroups of one XCD, which have neighbouring ranges, then read the same prefix.  The part of an item in one range is a segment; it leaves its
-// rows' maxima, sums and outputs in a slot of the workspace, and a second kernel joins the slots of a row.
+// next: workgroups of one XCD, which have neighbouring ranges, then read the same prefix (3 requests of 1024 tokens
+// behind 8192 keys: 432 us, 447 with a request's key heads one after another; 12 of 5 tokens: 26.9 and 29.8).  The
+// part of an item in one range is a segment; it leaves its rows' maxima, sums and outputs in a slot of the workspace,
+// and a second kernel joins the slots of a row.
 // Slot = item + range: both only grow along the list, one of them with every segment.
 //
 // Narrow tiles waste the matrix cores, wide ones the loads of rows that are not there: 16 rows are level (16 requests of 4
