@@ -11,7 +11,7 @@
 // 16-byte loads and stores in fp16), a workgroup one token's heads or a share of them, so the position, the
 // slot and the table row are uniform and the table's lines stay in the caches for all heads.  8192 tokens of 32 + 8 + 8
 // heads of 128 in fp16 (206 MB) are turned and stored in 41 us, 5.0 TB/s; 4093 tokens of 32 + 8 heads in fp32 (169 MB) are
-// turned in 38.6 us, 4.4 TB/s (a copy of 2 GiB moves 5.0).  Calls of a few tokens are the launch, 4.2 us.
+// turned in 35.6 us, 4.7 TB/s (a copy of 2 GiB moves 5.0).  Calls of a few tokens are the launch, 4.2 us.
 #include "gguf_common.h"
 #include "paged_launch.h"
 
@@ -74,10 +74,45 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a, int uni
   const float outside = position < 0 ? 0.0f : __builtin_nanf("");
   const float* row = a.angles + (size_t)(inside ? position : 0) * a.rotated;
   const float sign = a.inverse ? -1.0f : 1.0f;
-  if constexpr (VECTOR) {
+  if constexpr (VECTOR && INTERLEAVED) {
+    // 16 bytes at a time, the lanes of a head next to each other: a store then fills whole lines (4093 tokens of 40
+    // heads in fp32: 35.6 us, 38.6 with 64 bytes of each lane together)
+    constexpr int CH = 16 / sizeof(In), COUNT = 16 / CH;
+    typedef In Chunk __attribute__((ext_vector_type(CH)));
+    typedef Out ChunkOut __attribute__((ext_vector_type(CH)));
+    typedef float Half __attribute__((ext_vector_type(CH / 2)));
+    Chunk v[COUNT];
+    Half c[COUNT], s[COUNT];
+#pragma unroll
+    for (int k = 0; k < COUNT; ++k) {
+      const int i = CH * (unit + units * k);
+      v[k] = *reinterpret_cast<const Chunk*>(x + i);
+      if (!value && i < a.rotated) {
+        c[k] = *reinterpret_cast<const Half*>(row + i / 2);
+        s[k] = *reinterpret_cast<const Half*>(row + pairs + i / 2) * sign;
+      } else {
+        c[k] = 1.0f;
+        s[k] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < COUNT; ++k) {
+      const int i = CH * (unit + units * k);
+      const bool turned = !value && i < a.rotated;
+      ChunkOut to;
+#pragma unroll
+      for (int e = 0; e < CH; e += 2) {
+        const float x0 = (float)v[k][e], x1 = (float)v[k][e + 1], ce = c[k][e / 2], se = s[k][e / 2];
+        const float lo = turned ? x0 * ce - x1 * se : x0, hi = turned ? x1 * ce + x0 * se : x1;
+        to[e] = (Out)(value || inside ? lo : outside);
+        to[e + 1] = (Out)(value || inside ? hi : outside);
+      }
+      *reinterpret_cast<ChunkOut*>(out + i) = to;
+    }
+  } else if constexpr (VECTOR) {
     const bool turned = !value && unit < pairs / 8;
-    const int i = !turned || INTERLEAVED ? 16 * unit : 8 * unit;
-    const int j = !turned || INTERLEAVED ? i + 8 : i + pairs;
+    const int i = turned ? 8 * unit : 16 * unit;
+    const int j = turned ? i + pairs : i + 8;
     float v[16];
     load8(x + i, v);
     load8(x + j, v + 8);
@@ -87,11 +122,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a, int uni
       load8(row + pairs + 8 * unit, s);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float& lo = v[INTERLEAVED ? 2 * e : e];
-        float& hi = v[INTERLEAVED ? 2 * e + 1 : e + 8];
-        const float se = s[e] * sign, x0 = lo, x1 = hi;
-        lo = x0 * c[e] - x1 * se;
-        hi = x1 * c[e] + x0 * se;
+        const float se = s[e] * sign, x0 = v[e], x1 = v[e + 8];
+        v[e] = x0 * c[e] - x1 * se;
+        v[e + 8] = x1 * c[e] + x0 * se;
       }
     }
     if (!value && !inside) {
