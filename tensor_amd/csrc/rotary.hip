@@ -7,42 +7,16 @@
 // c and s come from a table of fp32 values, built once in 64 bits: positions reach 10^5 and more, where
 // a product in 32 bits is off by 0.004 radians, and every layer of a model reads the same rows.
 //
-// Bound by memory: each value is read and written once.  A thread moves 16 values of one head (two
-// 16-byte loads and stores in fp16), a workgroup one token's heads or a share of them, so the position, the
+// Bound by memory: each value is read and written once.  A thread moves 16 values of one head, 16
+// bytes at a time, a workgroup one token's heads or a share of them, so the position, the
 // slot and the table row are uniform and the table's lines stay in the caches for all heads.  8192 tokens of 32 + 8 + 8
-// heads of 128 in fp16 (206 MB) are turned and stored in 41 us, 5.0 TB/s; 4093 tokens of 32 + 8 heads in fp32 (169 MB) are
+// heads of 128 in fp16 (206 MB) are turned and stored in 40.4 us, 5.1 TB/s; 4093 tokens of 32 + 8 heads in fp32 (169 MB) are
 // turned in 35.6 us, 4.7 TB/s (a copy of 2 GiB moves 5.0).  Calls of a few tokens are the launch, 4.2 us.
 #include "gguf_common.h"
 #include "paged_launch.h"
 
 namespace tensor_paged {
 namespace {
-
-using tensor_gguf::half2_from_fp32;
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* v) {
-  if constexpr (sizeof(T) == 2) {
-    const tensor_gguf::half8_t h = *reinterpret_cast<const tensor_gguf::half8_t*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
-  } else {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float* v) {
-  if constexpr (sizeof(T) == 2) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(half2_from_fp32(v[0], v[1]), half2_from_fp32(v[2], v[3]),
-                                              half2_from_fp32(v[4], v[5]), half2_from_fp32(v[6], v[7]));
-  } else {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  }
-}
 
 // VECTOR: units of 16 values (dim and rotated multiples of 16); else units of one pair, or of one
 // value past the rotated dimensions, which any size takes (8192 tokens: 41 us and 92; 8 tokens: 4.5 and 5.3).
@@ -110,29 +84,49 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a, int uni
       *reinterpret_cast<ChunkOut*>(out + i) = to;
     }
   } else if constexpr (VECTOR) {
-    const bool turned = !value && unit < pairs / 8;
-    const int i = turned ? 8 * unit : 16 * unit;
-    const int j = turned ? i + pairs : i + 8;
-    float v[16];
-    load8(x + i, v);
-    load8(x + j, v + 8);
-    if (turned) {
-      float c[8], s[8];
-      load8(row + 8 * unit, c);
-      load8(row + pairs + 8 * unit, s);
+    // The same: units below `whole` take 8 pairs, in chunks among the others' of the first halves and the second ones;
+    // those from it on share what is not turned (4093 tokens of 40 heads in fp32: 33.3 us, 35.4 with 32 bytes of each
+    // lane together; half of each head turned: 35.2 and 38.4; 8192 stored in fp16: 40.4 and 41.8).
+    constexpr int CH = 16 / sizeof(In), COUNT = 16 / CH, HALF = COUNT / 2;
+    typedef In Chunk __attribute__((ext_vector_type(CH)));
+    typedef Out ChunkOut __attribute__((ext_vector_type(CH)));
+    typedef float Floats __attribute__((ext_vector_type(CH)));
+    const int whole = value ? 0 : pairs / 8;
+    const bool turned = unit < whole;
+    const int i = turned ? CH * unit : 16 * whole + CH * (unit - whole), apart = CH * (turned ? whole : units - whole);
+    const int second = turned ? pairs : HALF * apart;  // from a chunk to that HALF chunks later
+    Chunk v[COUNT];
+    Floats c[HALF], s[HALF];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float se = s[e] * sign, x0 = v[e], x1 = v[e + 8];
-        v[e] = x0 * c[e] - x1 * se;
-        v[e + 8] = x1 * c[e] + x0 * se;
+    for (int k = 0; k < HALF; ++k) {
+      v[k] = *reinterpret_cast<const Chunk*>(x + i + apart * k);
+      v[k + HALF] = *reinterpret_cast<const Chunk*>(x + i + apart * k + second);
+      if (turned) {
+#pragma unroll
+        for (int e = 0; e < CH; e += 4) {
+          const float4 cos = *reinterpret_cast<const float4*>(row + i + apart * k + e);
+          const float4 sin = *reinterpret_cast<const float4*>(row + pairs + i + apart * k + e);
+          c[k][e] = cos.x; c[k][e + 1] = cos.y; c[k][e + 2] = cos.z; c[k][e + 3] = cos.w;
+          s[k][e] = sin.x; s[k][e + 1] = sin.y; s[k][e + 2] = sin.z; s[k][e + 3] = sin.w;
+        }
+      } else {
+        c[k] = 1.0f;
+        s[k] = 0.0f;
       }
     }
-    if (!value && !inside) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = outside;
+    for (int k = 0; k < HALF; ++k) {
+      ChunkOut lo, hi;
+#pragma unroll
+      for (int e = 0; e < CH; ++e) {
+        const float x0 = (float)v[k][e], x1 = (float)v[k + HALF][e], se = s[k][e] * sign;
+        const float a0 = turned ? x0 * c[k][e] - x1 * se : x0, a1 = turned ? x1 * c[k][e] + x0 * se : x1;
+        lo[e] = (Out)(value || inside ? a0 : outside);
+        hi[e] = (Out)(value || inside ? a1 : outside);
+      }
+      *reinterpret_cast<ChunkOut*>(out + i + apart * k) = lo;
+      *reinterpret_cast<ChunkOut*>(out + i + apart * k + second) = hi;
     }
-    store8(out + i, v);
-    store8(out + j, v + 8);
   } else {
     if (unit >= pairs || value) {
       // past the pairs: one value a unit (a value row has one per unit from 0, two per unit below `pairs`)
