@@ -107,6 +107,11 @@ __device__ __forceinline__ float max16(float v) {
 // powers of two: weights stay below 2^8 in fp16, and most tiles rescale nothing (3 x 1024 tokens behind 8192 keys:
 // 416 us, 454 if every new maximum rescales).
 constexpr float kLazy = 8.0f;
+// A weight is exp2(s c - m c) in one operation, with m c rounded once for the row, or exp2((s - m) c) in two.  The rounding
+// scales all weights of a segment alike, but from this m c on by more than their own in fp16, and from 2^27 on by more than
+// fp16 holds: there wide segments take the second form, and narrow ones, whose time is the loads', everywhere
+// (3 x 1024 tokens behind 8192 keys: 386 us, 408 with the second form for every row).
+constexpr float kFar = 16384.0f;
 
 __device__ const uint4 zeros[1] = {};
 
@@ -336,6 +341,8 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
   }
   float16_t o[DB] = {};
   float m = -kInfinity, l = 0.0f, top;
+  float off = 0.0f;  // -m c, 0 before the first key
+  bool far = false;  // of some row of the wave: weights in two operations
   float s[16];  // scores, lane: row lane % 32, keys 8 (e / 4) + 4 half + e % 4
 
   // LDS addresses of this lane's fragments: a row of K in the tile at hand, its chunks; and four rows of V^T for
@@ -392,6 +399,8 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
       l *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] *= alpha;
+      off = m == -kInfinity ? 0.0f : -m * c;
+      far = __any(!(fabsf(off) < kFar));
     }
   };
   // weights of the scores in s, made from half HALF of a tile, with the scores of the next 32 keys (half 1 - HALF of
@@ -400,10 +409,16 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
   auto advance = [&](auto next, auto half_tile, int first, bool edge, uint32_t seen) {
     constexpr bool NEXT = decltype(next)::value;
     constexpr int HALF = decltype(half_tile)::value;
-    const float mc = m == -kInfinity ? 0.0f : m * c;
+    float add = off;
+    if (far) {
+      const float base = m == -kInfinity ? 0.0f : m;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] -= base;
+      add = 0.0f;
+    }
     uint32_t p[8];
     auto weigh = [&](int i) {  // two scores to weights; the sum is of the weights as the product takes them
-      const float2_t w = {__builtin_amdgcn_exp2f(s[2 * i] * c - mc), __builtin_amdgcn_exp2f(s[2 * i + 1] * c - mc)};
+      const float2_t w = {__builtin_amdgcn_exp2f(s[2 * i] * c + add), __builtin_amdgcn_exp2f(s[2 * i + 1] * c + add)};
       p[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(w, half2_t));
       l = dot2(p[i], 0x3C003C00u, l);
       asm volatile("" : "+v"(p[i]), "+v"(l));  // made here, not where they are used
@@ -662,11 +677,11 @@ __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Ext
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] *= alpha;
     }
-    const float mc = m == -kInfinity ? 0.0f : m * c;
+    const float base = m == -kInfinity ? 0.0f : m;
     uint32_t p[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2_t w = {__builtin_amdgcn_exp2f(s[2 * i] * c - mc), __builtin_amdgcn_exp2f(s[2 * i + 1] * c - mc)};
+      const float2_t w = {__builtin_amdgcn_exp2f((s[2 * i] - base) * c), __builtin_amdgcn_exp2f((s[2 * i + 1] - base) * c)};
       p[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(w, half2_t));
       l = dot2(p[i], 0x3C003C00u, l);
     }
