@@ -5,9 +5,9 @@
 // S^T = K Q^T (keys x rows) leaves the matrix cores with each lane holding scores of one row, so the softmax is
 // in-lane but for one or two exchanges, and the weights are the B operand of O^T += V^T P^T as they
 // are (the sum over keys takes them in any order, V^T's operand in the same).  Scores, m, l and O are fp32; the
-// weights are rounded to fp16 for the product (2^-11 of each, and l is the sum of the rounded ones).  K and V
-// tiles go to LDS by DMA, V^T comes out of it by transposing reads; chunks of 16 bytes are swizzled by row so that
-// both reads spread over the banks.
+// weights are rounded to fp16 for the product, 2^-11 of each, or 2^-32 of the largest where that is more (kLift); l is the
+// sum of the rounded ones.  K and V tiles go to LDS by DMA, V^T comes out of it by transposing reads; chunks of 16
+// bytes are swizzled by row so that both reads spread over the banks.
 //
 // Two kernels: `attend` leaves each segment's rows in a slot, `join_segments` adds up the slots of a row.
 //
@@ -104,13 +104,18 @@ __device__ __forceinline__ float max16(float v) {
   return fmaxf(a, b);
 }
 // The running maximum is raised (and the sums rescaled) only where a score passes it by this many
-// powers of two: weights stay below 2^8 in fp16, and most tiles rescale nothing (3 x 1024 tokens behind 8192 keys:
-// 416 us, 454 if every new maximum rescales).
+// powers of two: most tiles rescale nothing (3 x 1024 tokens behind 8192 keys: 416 us, 454 if every new maximum
+// rescales).
 constexpr float kLazy = 8.0f;
-// A weight is exp2(s c - m c) in one operation, with m c rounded once for the row, or exp2((s - m) c) in two.  The rounding
-// scales all weights of a segment alike, but from this m c on by more than their own in fp16, and from 2^27 on by more than
-// fp16 holds: there wide segments take the second form, and narrow ones, whose time is the loads', everywhere
-// (3 x 1024 tokens behind 8192 keys: 386 us, 408 with the second form for every row).
+// Weights are kept times 2^kLift, as are l and O, in every segment alike: up to 2^15 then, where fp16 ends at 2^16.  Below
+// 2^-14 fp16 keeps fewer bits and below 2^-25 none, so that keys which one key outweighs by 2^25 would be lost, however
+// many (131072 of them are 0.4% of the values); lifted, that is 2^32.
+constexpr float kLift = 7.0f;
+// A weight's exponent is s c + (kLift - m c) in one operation, the sum in brackets rounded once for the row, or
+// (s - m) c + kLift in two.  The rounding scales all weights of a segment alike, but from this m c on by more than
+// their own in fp16, and from 2^24 on by more than fp16 holds: there wide segments take the second form, and narrow
+// ones, whose time is the loads', everywhere (3 x 1024 tokens behind 8192 keys: 386 us, 408 with the second form for
+// every row).
 constexpr float kFar = 16384.0f;
 
 __device__ const uint4 zeros[1] = {};
@@ -341,7 +346,7 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
   }
   float16_t o[DB] = {};
   float m = -kInfinity, l = 0.0f, top;
-  float off = 0.0f;  // -m c, 0 before the first key
+  float off = kLift;  // kLift - m c; before the first key, kLift
   bool far = false;  // of some row of the wave: weights in two operations
   float s[16];  // scores, lane: row lane % 32, keys 8 (e / 4) + 4 half + e % 4
 
@@ -399,7 +404,7 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
       l *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] *= alpha;
-      off = m == -kInfinity ? 0.0f : -m * c;
+      off = m == -kInfinity ? kLift : kLift - m * c;
       far = __any(!(fabsf(off) < kFar));
     }
   };
@@ -414,7 +419,7 @@ __device__ __forceinline__ void wide_segment(const AttentionArgs& a, const Exten
       const float base = m == -kInfinity ? 0.0f : m;
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] -= base;
-      add = 0.0f;
+      add = kLift;
     }
     uint32_t p[8];
     auto weigh = [&](int i) {  // two scores to weights; the sum is of the weights as the product takes them
@@ -681,7 +686,8 @@ __device__ __forceinline__ void narrow_segment(const AttentionArgs& a, const Ext
     uint32_t p[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2_t w = {__builtin_amdgcn_exp2f((s[2 * i] - base) * c), __builtin_amdgcn_exp2f((s[2 * i + 1] - base) * c)};
+      const float2_t w = {__builtin_amdgcn_exp2f((s[2 * i] - base) * c + kLift),
+                          __builtin_amdgcn_exp2f((s[2 * i + 1] - base) * c + kLift)};
       p[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(w, half2_t));
       l = dot2(p[i], 0x3C003C00u, l);
     }
