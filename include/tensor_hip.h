@@ -283,6 +283,8 @@ int32_t tensor_gguf_dequant_v1(const TensorCallV1 *call, TensorErrorV1 *error);
 /*
  * One step's block tables and slot map from the requests' lengths.  Request b holds lengths[b] tokens
  * of its own and adds counts[b]; pages it lacks come off the end of the free list, in request order.
+ * table_out may be table itself; an output that shares other memory with a buffer of the call is refused: the
+ * rest of the state goes from step to step through two sets of buffers, or a copy.
  * Arguments, in order:
  *    0 lengths     int32 [B]     tokens held (negative: as 0)
  *    1 counts      int32 [B]     new tokens (negative: as 0)

@@ -46,6 +46,33 @@ int32_t check_ints(const TensorArgumentV1& arg, const char* name, int ordinal, i
   return TENSOR_OK;
 }
 
+// A buffer that a call writes: its argument, and the one (-1: none) that it may be itself, whose every value is read by
+// the thread that writes it.
+struct Written {
+  int at;
+  const char* name;
+  int twin;
+};
+
+// Written buffers share no memory with the call's others, which other workgroups may not have read yet.
+template <size_t N>
+int32_t check_apart(const TensorCallV1* call, const Written (&written)[N], TensorErrorV1* error) {
+  auto bytes = [&](uint32_t i) {
+    const TensorBufferV1& b = call->arguments[i].buffer;
+    return (uint64_t)b.shape[0] * (uint64_t)b.strides[0];  // contiguous (check_buffer)
+  };
+  for (const Written& w : written) {
+    const uint64_t from = call->arguments[w.at].buffer.address, to = from + bytes(w.at);
+    for (uint32_t i = 0; i < call->argument_count; ++i) {
+      if ((int)i == w.at || call->arguments[i].kind != TENSOR_ARG_BUFFER) continue;
+      const uint64_t other = call->arguments[i].buffer.address, end = other + bytes(i);
+      if (end <= from || to <= other || ((int)i == w.twin && other == from && end == to)) continue;
+      return fail(error, TENSOR_ERROR_ARGUMENT, "%s: written, and shares memory with argument %u", w.name, i);
+    }
+  }
+  return TENSOR_OK;
+}
+
 // log2 of a page size: a power of two from 1 to 1024 tokens; -1 otherwise
 int page_shift(int64_t size) {
   for (int shift = 0; shift <= 10; ++shift)
@@ -87,6 +114,9 @@ int32_t slots_call(const TensorCallV1* call, TensorErrorV1* error) {
   CHECK(check_ints(a[10], "slots", ordinal, tokens, 1, error));
   CHECK(check_ints(a[11], "table_out", ordinal, table, 2, error));
   CHECK(check_ints(a[12], "free_left", ordinal, one, 1, error));
+  // Every workgroup sums the earlier requests' lengths and counts; only the table's entries are each one's own.
+  CHECK(check_apart(call, {{7, "offsets", -1}, {8, "lengths_out", -1}, {9, "positions", -1}, {10, "slots", -1},
+                           {11, "table_out", 5}, {12, "free_left", -1}}, error));
   CHECK(check_device(call, error));
   tensor_paged::SlotsArgs args{};
   args.lengths = pointer<const int32_t>(a[0]);
