@@ -277,14 +277,14 @@ int32_t tensor_gguf_dequant_v1(const TensorCallV1 *call, TensorErrorV1 *error);
  * slot is page * page_size + place in the page.  A request's own tokens fill the pages of its table
  * row in order; tokens that all requests share (a common prompt) may stand before them, in pages of
  * a list of their own.  Lengths, counts, tables and lists are read on the device: a captured graph
- * follows them as they grow.  int32 buffers need 4-byte alignment, the others 16.
+ * follows them as they grow.  int32 buffers need 4-byte alignment, the others 16.  A call refuses a
+ * buffer that it writes and that shares memory with another of its buffers, except where it says that the two may be one.
  */
 
 /*
  * One step's block tables and slot map from the requests' lengths.  Request b holds lengths[b] tokens
  * of its own and adds counts[b]; pages it lacks come off the end of the free list, in request order.
- * table_out may be table itself; an output that shares other memory with a buffer of the call is refused: the
- * rest of the state goes from step to step through two sets of buffers, or a copy.
+ * table_out may be table itself; the rest of the state goes from step to step through two sets of buffers, or a copy.
  * Arguments, in order:
  *    0 lengths     int32 [B]     tokens held (negative: as 0)
  *    1 counts      int32 [B]     new tokens (negative: as 0)
@@ -310,7 +310,7 @@ int32_t tensor_paged_slots_v1(const TensorCallV1 *call, TensorErrorV1 *error);
  * token's position in `angles`; dimensions past `rotated` are copied.  Pairs are (p, p + rotated / 2)
  * (layout 0) or (2 p, 2 p + 1) (layout 1).  inverse = 1 turns back, which is also the gradient of the
  * forward call.  A token of negative position (padding) gives zeros, one past the table NaN.
- *    0 q         fp16 or fp32 [T, heads, dim]        4 q_out  as q
+ *    0 q         fp16 or fp32 [T, heads, dim]        4 q_out  as q (may be q, and k_out k)
  *    1 k         same dtype [T, kv_heads, dim]       5 k_out  as k
  *    2 positions int32 [T]                           6 layout scalar uint32
  *    3 angles    fp32 [reach, rotated]: rotated / 2 cosines, then as many sines    7 inverse scalar uint32
@@ -323,7 +323,7 @@ int32_t tensor_rotary_v1(const TensorCallV1 *call, TensorErrorV1 *error);
  * of one slot are the caller's error.
  *    0 q, 1 k, 2 v  fp16 or fp32 (one dtype) [T, heads, dim], [T, kv_heads, dim], [T, kv_heads, dim]
  *    3 positions int32 [T]    4 slots int32 [T]    5 angles fp32 [reach, rotated]
- *    6 q_out fp16 [T, heads, dim]    7 k_cache, 8 v_cache: updated in place    9 layout scalar uint32
+ *    6 q_out fp16 [T, heads, dim] (may be an fp16 q)    7 k_cache, 8 v_cache: updated in place    9 layout scalar uint32
  */
 int32_t tensor_rotary_store_v1(const TensorCallV1 *call, TensorErrorV1 *error);
 
@@ -344,7 +344,7 @@ int32_t tensor_rotary_store_v1(const TensorCallV1 *call, TensorErrorV1 *error);
  *    7 prefix_length int32 [1]      its keys (0: none)
  *    8 workspace     uint8 [bytes]  256-byte aligned device scratch, clobbered; at least what
  *                                   tensor_paged_attention_workspace_v1 tells; not for two calls at once
- *    9 out           fp16 [T, heads, dim]
+ *    9 out           fp16 [T, heads, dim]  (may be q)
  *   10 scale         scalar fp32, 0 for 1 / sqrt(dim)
  */
 int32_t tensor_paged_attention_v1(const TensorCallV1 *call, TensorErrorV1 *error);

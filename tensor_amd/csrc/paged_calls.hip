@@ -180,6 +180,7 @@ int32_t rotary_call(const TensorCallV1* call, TensorErrorV1* error, bool store) 
     args.page_shift = page_shift(cache[2]);
     if (args.page_shift < 0 || cache[0] >= (int64_t)1 << 31)
       return fail(error, TENSOR_ERROR_ARGUMENT, "k_cache: pages of a power of two from 1 to 1024 tokens");
+    CHECK(check_apart(call, {{6, "q_out", 0}, {7, "k_cache", -1}, {8, "v_cache", -1}}, error));
     args.pages = (int)cache[0];
     args.v = pointer<const void>(a[2]);
     args.slots = pointer<const int32_t>(a[4]);
@@ -187,6 +188,7 @@ int32_t rotary_call(const TensorCallV1* call, TensorErrorV1* error, bool store) 
     args.v_out = pointer<void>(a[8]);
   } else {
     CHECK(check_buffer(a[5], "k_out", ordinal, out_dtype, k, 3, 16, error));
+    CHECK(check_apart(call, {{4, "q_out", 0}, {5, "k_out", 1}}, error));
     args.k_out = pointer<void>(a[5]);
   }
   CHECK(check_device(call, error));
@@ -274,6 +276,7 @@ int32_t attention_call(const TensorCallV1* call, TensorErrorV1* error) {
   if ((uint64_t)workspace[0] < need)
     return fail(error, TENSOR_ERROR_ARGUMENT, "workspace: the call needs %zu bytes, %lld available", need,
                 (long long)workspace[0]);
+  CHECK(check_apart(call, {{8, "workspace", -1}, {9, "out", 0}}, error));  // (a row's segment reads its queries first)
   CHECK(check_device(call, error));
   args.q = pointer<const void>(a[0]);
   args.k_cache = pointer<const void>(a[1]);

@@ -5,8 +5,9 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+from tensor_amd.kernels.paged import rotary_angles
 from tests import paged_cases as plain
-from tests.test_gpu_paged import Buffers
+from tests.test_gpu_paged import Buffers, make, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +41,35 @@ def test_slots_refuse_their_other_inputs_as_outputs(hip_device):
             with pytest.raises(Exception, match="shares memory"):
                 kernel.launch(*ins, 2, *mixed)
         assert [b.to_numpy().tolist() for b in ins] == [[3, 1], [1, 1], [0], [5, 6], [2], [[0, -1], [1, -1]]]
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dim,rotated", [(128, 128), (64, 32), (96, 46)])
+def test_store_turns_queries_in_place(hip_device, dim, rotated, layout):
+    rng = np.random.default_rng(dim)
+    tokens, heads, kv = 37, 6, 2
+    q, k, v = (rng.standard_normal((tokens, n, dim)).astype(np.float16) for n in (heads, kv, kv))
+    at, slots = rng.integers(0, 90, tokens).astype(np.int32), rng.permutation(48)[:tokens].astype(np.int32)
+    with Buffers(hip_device) as put:
+        kernel = hip_device.load("rotary_store", layout=layout)
+        shared = [put(x) for x in (q, k, v, at, slots, rotary_angles(90, rotated))]
+        caches = [put(np.zeros((3, kv, 16, dim), np.float16)) for _ in range(2)]
+        apart = put.empty(q.shape, "float16")
+        kernel.launch(*shared, apart, *caches)
+        kernel.launch(*shared, shared[0], *caches)
+        assert np.array_equal(apart.to_numpy(), shared[0].to_numpy())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv", [(8, 2), (7, 1), (32, 1)])
+def test_attention_writes_over_its_queries(hip_device, heads, kv, dim):
+    """Requests of one segment, which write their rows themselves, and of many, which are joined."""
+    rng = np.random.default_rng(heads + dim)
+    for counts, lengths, prefix in (([1, 3, 40, 1], [9, 300, 150, 30], 0), ([1, 200, 2], [1, 200, 900], 70), ([130], [400], 0)):
+        call = make(rng, counts, lengths, prefix, heads, kv, dim, 16, padding=2)
+        want = run_attention(hip_device, *call)
+        with Buffers(hip_device) as put:
+            ins = [put(x) for x in call[:7]] + [put(np.array([prefix], np.int32))]
+            need = hip_device.attention_workspace(len(call[0]), len(counts), heads, kv, dim)
+            hip_device.load("paged_attention").launch(*ins, put.empty((need,), "uint8"), ins[0])
+            assert np.array_equal(ins[0].to_numpy().astype(np.float64), want)

@@ -5,16 +5,19 @@ from __future__ import annotations
 
 import pytest
 
-from tests.test_paged import CALLS, ERR_ARG, ERR_PROVIDER
+from tensor_amd.kernels import builtin
+from tests.test_paged import CALLS, ERR_ARG, ERR_PROVIDER, Call
 
 # written argument -> the input that it may be itself
 WRITTEN = {"slots": {"offsets": None, "lengths_out": None, "positions": None, "slots": None, "table_out": "table",
-                     "free_left": None}}
+                     "free_left": None},
+           "rotary": {"q_out": "q", "k_out": "k"}, "store": {"q_out": "q", "k_cache": None, "v_cache": None},
+           "attention": {"workspace": None, "out": "q"}}
 
 
-def spread(kind):
+def spread(kind, call=None):
     """A call whose buffers share nothing, on a device that no machine has: past the checks it ends there."""
-    call = CALLS[kind]()
+    call = call or CALLS[kind]()
     call.call.stream.device_ordinal = 1 << 20
     for i, arg in enumerate(call.args):
         if arg.kind == 1:
@@ -60,3 +63,14 @@ def test_shared_memory_is_refused(kind):
                 assert status == (ERR_PROVIDER if allowed else ERR_ARG), (name, other, part, message)
                 if not allowed:
                     assert "shares memory" in message and (name in message or other in message), message
+
+
+def test_fp16_queries_do_not_go_into_the_fp32_ones():
+    """rotary_store rounds its queries: in place, a token's would lie over another's that is still to be read."""
+    shapes = dict(q=(3, 8, 64), k=(3, 2, 64), v=(3, 2, 64), positions=(3,), slots=(3,), angles=(10, 32), q_out=(3, 8, 64),
+                  k_cache=(5, 2, 16, 64), v_cache=(5, 2, 16, 64))
+    call = spread("store", Call(builtin.manifest("rotary_store", dtype="float32"), shapes, {}))
+    assert call.run()[0] == ERR_PROVIDER
+    call.args[call.index["q_out"]].buffer.address = call.args[call.index["q"]].buffer.address
+    status, message = call.run()
+    assert status == ERR_ARG and "shares memory" in message
