@@ -214,4 +214,6 @@ def manifest(kernel: str, encoding, out_dtype: str | None = None, count: int | N
         result["shape_domain"] = {"M": [1, GEMV_MAX_M]}
     if kernel == "gguf_gemv_variant":
         result["shape_domain"] = {"M": [2, GEMV_MAX_M]}
+    if any(item["name"] == "workspace" for item in arguments):
+        result["scratch"] = ["workspace"]
     return result

@@ -124,7 +124,7 @@ def attention_manifest(*, scale: float | None = None) -> dict:
     return _result("paged_attention", "default" if scale is None else str(float(scale)), arguments, ["out"],
                    "T H G D N L B P PP W", {"scale": 0.0 if scale is None else float(scale)},
                    shape_domain={"D": [min(HEAD_DIMS), max(HEAD_DIMS)], "B": [1, MAX_REQUESTS]},
-                   shape_divisors={"D": 64})
+                   shape_divisors={"D": 64}, scratch=["workspace"])
 
 
 _MANIFESTS = {"paged_slots": slots_manifest, "rotary": rotary_manifest, "rotary_store": rotary_store_manifest,

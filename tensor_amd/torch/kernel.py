@@ -9,11 +9,13 @@ mutation form that writes caller-owned outputs.
 
 Artifacts are the HIP provider's: a built-in kernel by name with its
 options (``Kernel("gguf_linear", encoding="q4_k")``), a manifest dict, or a
-``hip`` bundle by path.  Input buffers must be read-only in the kernel and
-declared outputs completely written, never aliasing inputs (the functional
-custom-operator contract); ``mutable_inputs`` names input buffers a kernel
-without declared outputs writes, which ``raw`` and ``prepare`` launch (a
-built-in kernel's manifest names its own).
+``hip`` bundle by path.  Input buffers must be read-only in the kernel, but
+for those that its manifest names as ``scratch`` (a workspace: the registered
+operator declares that it writes them), and declared outputs completely
+written, never aliasing inputs (the functional custom-operator contract);
+``mutable_inputs`` names input buffers a kernel without declared outputs
+writes, which ``raw`` and ``prepare`` launch (a built-in kernel's manifest
+names its own).
 """
 
 from __future__ import annotations
@@ -76,6 +78,9 @@ class Kernel:
         if len(set(self.mutable_inputs)) != len(self.mutable_inputs) or set(self.mutable_inputs) - {
                 d["name"] for d in self.inputs if buffer_argument(d)}:
             raise ValueError("mutable_inputs must name distinct input buffers")
+        self.scratch = tuple(self.manifest.get("scratch", ()))
+        if set(self.scratch) - {d["name"] for d in self.inputs if buffer_argument(d)}:
+            raise ValueError("scratch must name input buffers")
         self._slots = _slots(self.manifest)
         self._executables: dict = {}
         self._prepared: OrderedDict = OrderedDict()
@@ -148,18 +153,30 @@ class Kernel:
     def register(self):
         return register(self)
 
+    def _group(self, descriptor):
+        """The list of the registered operator's that an input is in: tensors, scratch (if any), scalars."""
+        if not buffer_argument(descriptor):
+            return 2 if self.scratch else 1
+        return int(descriptor["name"] in self.scratch)
+
+    def _groups(self, args):
+        groups = [[] for _ in range(3 if self.scratch else 2)]
+        for descriptor, value in zip(self.inputs, args):
+            groups[self._group(descriptor)].append(value)
+        return groups
+
     def __call__(self, *args):
         op = self._op or self.register()
-        result = op([v for d, v in zip(self.inputs, args) if buffer_argument(d)],
-                    [v for d, v in zip(self.inputs, args) if not buffer_argument(d)])
+        result = op(*self._groups(args))
+        if isinstance(result, torch.Tensor):
+            return result
         return result[0] if len(result) == 1 else tuple(result)
 
     def into(self, *args, outputs):
         """Write caller-owned, disjoint outputs through the registered mutation operator."""
         if self._into_op is None:
             self.register()
-        self._into_op([v for d, v in zip(self.inputs, args) if buffer_argument(d)],
-                      [v for d, v in zip(self.inputs, args) if not buffer_argument(d)], list(outputs))
+        self._into_op(*self._groups(args), list(outputs))
 
 
 def register(kernel):
@@ -171,27 +188,38 @@ def register(kernel):
     # Each load is its own operator, even for the same artifact.
     name = f"kernel_{hashlib.sha256(kernel._identity).hexdigest()[:16]}_{next(_operator_ids)}"
 
-    def unpack(tensors, scalars):
-        tensors, scalars = iter(tensors), iter(scalars)
-        return tuple(next(tensors) if buffer_argument(d) else next(scalars) for d in kernel.inputs)
+    def unpack(*groups):
+        groups = [iter(group) for group in groups]
+        return tuple(next(groups[kernel._group(d)]) for d in kernel.inputs)
 
-    @torch.library.custom_op("tensor_amd::" + name, mutates_args=(),
-                             schema="(Tensor[] tensors, Scalar[] scalars) -> Tensor[]")
-    def op(tensors, scalars):
-        return kernel._run(unpack(tensors, scalars))
+    # An operator that writes one of its inputs returns a fixed number of tensors, not a list: torch.compile does not
+    # make such an operator functional.
+    scratch, returned = bool(kernel.scratch), "Tensor[]"
+    inputs = "Tensor[] tensors, Tensor(a!)[] scratch, Scalar[] scalars" if scratch else "Tensor[] tensors, Scalar[] scalars"
+    if scratch:
+        returned = f"({', '.join(['Tensor'] * len(kernel.outputs))})"
+
+    def results(outputs):
+        return outputs if not scratch else outputs[0] if len(outputs) == 1 else tuple(outputs)
+
+    @torch.library.custom_op("tensor_amd::" + name, mutates_args={"scratch"} if scratch else (),
+                             schema=f"({inputs}) -> {returned}")
+    def op(*groups):
+        return results(kernel._run(unpack(*groups)))
 
     @op.register_fake
-    def _(tensors, scalars):
-        return kernel.fake(unpack(tensors, scalars))
+    def _(*groups):
+        return results(kernel.fake(unpack(*groups)))
 
-    @torch.library.custom_op("tensor_amd::" + name + "_into", mutates_args={"outputs"},
-                             schema="(Tensor[] tensors, Scalar[] scalars, Tensor(a!)[] outputs) -> ()")
-    def into(tensors, scalars, outputs):
-        kernel._launch(unpack(tensors, scalars), outputs)
+    @torch.library.custom_op("tensor_amd::" + name + "_into", mutates_args={"scratch", "outputs"} if scratch else {"outputs"},
+                             schema=f"({inputs}, Tensor({'b' if scratch else 'a'}!)[] outputs) -> ()")
+    def into(*groups):
+        kernel._launch(unpack(*groups[:-1]), groups[-1])
 
     @into.register_fake
-    def _(tensors, scalars, outputs):
-        expected = kernel.fake(unpack(tensors, scalars))
+    def _(*groups):
+        *groups, outputs = groups
+        expected = kernel.fake(unpack(*groups))
         if len(expected) != len(outputs):
             raise ValueError("wrong output count")
         for want, out in zip(expected, outputs):
