@@ -308,8 +308,9 @@ int32_t tensor_paged_slots_v1(const TensorCallV1 *call, TensorErrorV1 *error);
 /*
  * Rotary positions: the pair (a, b) of dimensions becomes (a c - b s, b c + a s), c and s the row of the
  * token's position in `angles`; dimensions past `rotated` are copied.  Pairs are (p, p + rotated / 2)
- * (layout 0) or (2 p, 2 p + 1) (layout 1).  inverse = 1 turns back, which is also the gradient of the
- * forward call.  A token of negative position (padding) gives zeros, one past the table NaN.
+ * (layout 0) or (2 p, 2 p + 1) (layout 1).  inverse = 1 takes -s: the transposed map, which is the forward call's
+ * gradient whatever the table, and turns back where c^2 + s^2 = 1 (a table scaled by f gives f^2 times the input).
+ * A token of negative position (padding) gives zeros, one past the table NaN.
  *    0 q         fp16 or fp32 [T, heads, dim]        4 q_out  as q (may be q, and k_out k)
  *    1 k         same dtype [T, kv_heads, dim]       5 k_out  as k
  *    2 positions int32 [T]                           6 layout scalar uint32

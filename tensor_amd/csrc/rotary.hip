@@ -2,8 +2,8 @@
 // cache, one launch:
 //   (a, b) -> (a c - b s, b c + a s), c and s the cosine and sine of the token's position times the
 //   pair's frequency, for the leading `rotated` dimensions of every head; pairs are dimensions
-//   (p, p + rotated / 2) or (2 p, 2 p + 1); the inverse rotation takes -s (the rotation is orthogonal:
-//   it is also the gradient of the forward one).
+//   (p, p + rotated / 2) or (2 p, 2 p + 1); the inverse takes -s: the transposed map, the gradient of the forward one
+//   whatever c and s, and its inverse where c^2 + s^2 = 1.
 // c and s come from a table of fp32 values, built once in 64 bits: positions reach 10^5 and more, where
 // a product in 32 bits is off by 0.004 radians, and every layer of a model reads the same rows.
 //

@@ -4,7 +4,7 @@ They stand between a layer's q + k + v linears and its output linear and are loa
 GGUF kernels are (``Device.load``, ``tensor_amd.torch.load``):
 
 * ``paged_slots`` (``page_size``): a step's block tables, slots and positions from request lengths;
-* ``rotary`` (``layout``, ``dtype``, ``inverse``): rotary positions of queries and keys;
+* ``rotary`` (``layout``, ``dtype``, ``inverse``): rotary positions of queries and keys, or their gradient;
 * ``rotary_store`` (``layout``, ``dtype``): the same, keys and values written to their cache slots;
 * ``paged_attention`` (``scale``): attention over a shared prefix and each request's own pages.
 
@@ -151,7 +151,7 @@ def rotary_angles(reach: int, rotated: int, *, base: float = 10000.0, scaling: s
     * ``ntk``: the base raised so that the slowest pair is slowed by the factor and the fastest kept;
     * ``yarn``: pairs that turn more than ``fast`` times in ``original`` positions kept, those that turn less
       than ``slow`` times slowed by the factor, a ramp over the pairs between, and cosines and sines scaled by
-      0.1 ln(factor) + 1.
+      f = 0.1 ln(factor) + 1 (``rotary`` with ``inverse`` after ``rotary`` gives f^2 times its input then).
     """
     if type(reach) is not int or type(rotated) is not int or reach < 1 or rotated < 2 or rotated % 2:
         raise ValueError("reach must be a positive integer and rotated a positive even one")
