@@ -294,7 +294,7 @@ int32_t tensor_gguf_dequant_v1(const TensorCallV1 *call, TensorErrorV1 *error);
  *    5 table       int32 [B, P]  page of each page_size tokens of a request, -1 past its last
  *    6 T           scalar int32  rows of the token outputs, at least the sum of counts
  *    7 offsets     int32 [B + 1] out: first row of each request's tokens, then their number
- *    8 lengths_out int32 [B]     out: lengths + counts
+ *    8 lengths_out int32 [B]     out: lengths + counts (like the next and the last, held at int32's ends)
  *    9 positions   int32 [T]     out: start + place in the request; -1 past the last token
  *   10 slots       int32 [T]     out: slot; -1 past the last token, for a token without a page and for a
  *                                 page whose slots pass int32

@@ -18,6 +18,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Sums past int32 stop at its ends: a wrapped length would be none, a wrapped position padding.
+__device__ __forceinline__ int saturated(int64_t v) { return (int)max(min(v, (int64_t)INT32_MAX), (int64_t)INT32_MIN); }
+
 __global__ __launch_bounds__(kThreads) void paged_slots(const SlotsArgs a) {
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int S = 1 << a.page_shift;
@@ -65,11 +68,11 @@ __global__ __launch_bounds__(kThreads) void paged_slots(const SlotsArgs a) {
     const int32_t p = column < a.columns ? page((int)column) : -1;
     // (a page whose slots pass 31 bits has none: a wrapped one would be another page's)
     a.slots[tokens + i] = p < 0 || p >> (31 - a.page_shift) ? -1 : (p << a.page_shift) + (int)(place & (S - 1));
-    a.positions[tokens + i] = (int)(start + place);
+    a.positions[tokens + i] = saturated(start + place);
   }
   if (blockIdx.y == 0 && tid == 0) {
     a.offsets[b] = (int)min(tokens, (int64_t)a.tokens);
-    a.lengths_out[b] = (int)(l + n);
+    a.lengths_out[b] = saturated(l + n);
   }
   if (b == a.requests - 1) {
     const int64_t all = tokens + n;
@@ -79,7 +82,7 @@ __global__ __launch_bounds__(kThreads) void paged_slots(const SlotsArgs a) {
     }
     if (blockIdx.y == 0 && tid == 0) {
       a.offsets[a.requests] = (int)min(all, (int64_t)a.tokens);
-      *a.free_left = (int)(available - (pages + wanted - held));
+      *a.free_left = saturated(available - (pages + wanted - held));
     }
   }
 }
