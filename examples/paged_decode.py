@@ -52,6 +52,7 @@ class Layer:
         self.slots = tensor_torch.load("paged_slots", page_size=page)
         self.store = tensor_torch.load("rotary_store", layout="half")
         self.attention = tensor_torch.load("paged_attention")
+        self.workspace = None  # of the attention, as large as a step has needed
 
     def project(self, x):
         return [self.linear(x, self.weights[name]).view(x.shape[0], -1, self.dim) for name in "qkv"]
@@ -65,8 +66,9 @@ class Layer:
         turned = torch.empty_like(q)
         self.store.raw(q, k, v, positions, slots, self.angles, turned, self.k_cache, self.v_cache)
         need = session(x.device.index).attention_workspace(tokens, requests, self.heads, self.kv, self.dim)
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-        a = self.attention(turned, self.k_cache, self.v_cache, offsets, lengths, table, prefix_pages, start, workspace)
+        if self.workspace is None or self.workspace.numel() < need:
+            self.workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+        a = self.attention(turned, self.k_cache, self.v_cache, offsets, lengths, table, prefix_pages, start, self.workspace)
         return self.linear(a.view(tokens, -1), self.weights["o"]), a, lengths, table
 
 
