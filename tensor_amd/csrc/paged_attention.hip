@@ -104,7 +104,7 @@ __device__ __forceinline__ float max16(float v) {
   return fmaxf(a, b);
 }
 // The running maximum is raised (and the sums rescaled) only where a score passes it by this many
-// powers of two: most tiles rescale nothing (3 x 1024 tokens behind 8192 keys: 416 us, 454 if every new maximum
+// powers of two: most tiles rescale nothing (3 x 1024 tokens behind 8192 keys: 386 us, 432 if every new maximum
 // rescales).
 constexpr float kLazy = 8.0f;
 // Weights are kept times 2^kLift, as are l and O, in every segment alike: up to 2^15 then, where fp16 ends at 2^16.  Below
@@ -217,7 +217,8 @@ struct Keys {
 // A wave's rows of a tile, GROUPS times 16.  Where all its pages are there and hold 16 tokens or more, a group's
 // rows lie one after another, and where is in scalar registers (those of a page that are past the last key are
 // loaded too; a group past it is the last one again).  Otherwise each row is looked up, and a key that is not there
-// read as zeros.
+// read as zeros (pages of 8 tokens: 405 us for 256 requests of up to 4096 keys, 398 with pages of 16; 3 x 1024 tokens behind
+// 8192 keys: 514 and 386).
 template <int D, int COUNT, int GROUPS>
 struct Rows {
   static constexpr int CH = D / 8, RPI = 512 / D, PER = D / 32;  // chunks of a row, rows of a load, loads of a group
@@ -919,9 +920,9 @@ __global__ __launch_bounds__(kThreads, 2) void attend(const AttentionArgs a) {
 // are added up through LDS.  A segment's maximum and sum are in one lane each, so that a lane computes one
 // weight for all dimensions and the outputs' loads wait for nothing but the record.
 //
-// Bound by the slots' bytes in large calls (3 x 1024 tokens: 68 MB in and 17 out of 98304 rows, 28-35 us, 13-15 of it
-// the workgroups' own start and index arithmetic) and by its chain of loads in small ones (5.5 us).  Four outputs in flight
-// a lane: eight take more registers, and 44 us there.
+// Bound by the slots' bytes in large calls (3 x 1024 tokens: 68 MB in and 17 out of 98304 rows, 28-34 us, much of it
+// the workgroups' own start and index arithmetic) and by its chain of loads in small ones (5.5-6 us).  Four outputs in
+// flight a lane: eight take more registers (392 us for that call, 386 with four; a prompt of 4096 tokens: 213 and 206).
 template <int D, int THREADS>
 __global__ __launch_bounds__(THREADS) void join_segments(const AttentionArgs a, int split) {
   constexpr int LANES = D / 4, SETS = THREADS / LANES, BATCH = 4;
@@ -1019,7 +1020,8 @@ hipError_t launch_dim(const AttentionArgs& a, hipStream_t stream) {
   hipError_t status = hipGetLastError();
   if (status != hipSuccess) return status;
   // Few rows: more sets of lanes for each, to 8192 or more in all (64 requests behind 16384 keys, 2048 rows of 34
-  // segments: 58 us for the call, at 2048 sets as well, at 32768 69; one token: 12.9, 13.2, 13.0).
+  // segments: 56 us for the call, at 2048 sets as well, at 32768 65; with heads of 64: 34.6, 35.7, 38.5; 32 requests of up to
+  // 2000 keys: 37.9, 37.1, 41.2).
   constexpr int lanes = D / 4;
   const int rows = a.tokens * a.heads;
   int split = 1;

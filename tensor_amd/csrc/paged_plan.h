@@ -8,22 +8,23 @@
 // which those of the second half of the workgroups take more where the first has wide work.  A range crosses
 // items, so the work is even whatever the lengths.  A list goes through all requests for one key head before the
 // next: workgroups of one XCD, which have neighbouring ranges, then read the same prefix (3 requests of 1024 tokens
-// behind 8192 keys: 432 us, 447 with a request's key heads one after another; 12 of 5 tokens: 26.9 and 29.8).  The
+// behind 8192 keys: 383 us, 395 with a request's key heads one after another; 12 of 5 tokens: 26.2 and 28.8).  The
 // part of an item in one range is a segment; it leaves its rows' maxima, sums and outputs in a slot of the workspace,
 // and a second kernel joins the slots of a row.
 // Slot = item + range: both only grow along the list, one of them with every segment.
 //
 // Narrow tiles waste the matrix cores, wide ones the loads of rows that are not there: 16 rows are level (16 requests of 4
-// tokens and 4 heads a key head, 16000 keys: 208 us narrow, 204 wide; 1000 keys: 66 and 65), and fewer stay narrow.
+// tokens and 4 heads a key head, 16000 keys: 203 us narrow, 196 wide; 1000 keys: 25.2 and 26.3), and fewer stay narrow.
 //
 // To begin a wide item costs a workgroup as much as kItemCost tiles, so where there is an item for every fourth
-// workgroup each has that many empty positions before its first tile (a prompt of 1024 tokens: 45 us, 56 without; 16
-// requests of 33 tokens behind 8192 keys: 123 and 156; but 64 requests behind 16384 keys, 16 items: 62 and 59).
+// workgroup each has that many empty positions before its first tile (a prompt of 1024 tokens: 43 us, 54 without; of 512,
+// where a range is shorter than that and some hold no tile: 28.3 and 30.2; 16 requests of 33 tokens behind 8192 keys: 108
+// and 232; but 64 requests behind 16384 keys, 16 items: 59 and 56).
 //
 // The prefix is a list entry of its own where tokens of several requests fill its row tiles; where each request
 // fills tiles of its own (prompts, one request), its wide items begin with the prefix's tiles instead (`lead`),
-// which leaves one slot less to write and join (3 requests of 1024 tokens behind 8192 keys: 422 us, 447 apart; 8 of 128
-// behind 4096: 114 and 129; but 16 of 33 behind 8192, whose tiles would be half empty: 173, and 121 apart).
+// which leaves one slot less to write and join (3 requests of 1024 tokens behind 8192 keys: 386 us, 417 apart; 8 of 128
+// behind 4096: 104 and 116; but 16 of 33 behind 8192, whose tiles would be half empty: 130, and 108 apart).
 #pragma once
 
 #include <stddef.h>
@@ -263,15 +264,16 @@ struct Quota {
   }
 };
 // A short list beside a narrow one goes to half the workgroups, one on a CU, whose other one reads the narrow list's
-// keys meanwhile, and leaves half the slots (64 requests behind 16384 keys: 59 us, 72 with all; 12 requests of 5 tokens:
-// 29.6 and 33.7).  A long one needs all (3 x 1024 tokens: 425 us, 499 with half), and so does one alone (a prompt of
-// 1024 tokens: 56 us, 63 with half).
+// keys meanwhile, and leaves half the slots (64 requests behind 16384 keys: 56 us, 69 with all; 12 requests of 5 tokens:
+// 26.2 and 30.3).  A long one needs all (3 x 1024 tokens: 386 us, 458 with half), and so does one alone (a prompt of
+// 4096 tokens: 206 us, 244 with half; of 1024: 43 and 45; of 512: 28.3 and 26.9).
 PAGED_CODE Quota wide_quota(int positions, int narrow) {
   const int ranges = narrow && positions < kLongRange * kGroups ? kGroups / 2 : kGroups;
   return Quota{(positions + ranges - 1) / ranges, -1};
 }
 // `wide`: positions of a wide range.  While the first half of the workgroups have those, the others take kBeside
-// narrow tiles for each; the rest is for all (64 requests behind 16384 keys: 57 us, 65 in equal shares).
+// narrow tiles for each; the rest is for all (64 requests behind 16384 keys: 56 us, 63 in equal shares; with
+// heads of 64, whose narrow tiles are half the bytes: 35 and 41).
 PAGED_CODE Quota narrow_quota(int positions, int wide) {
   const int few = (int)(most64(positions - (int64_t)kBeside * wide, 0) / kStreams);
   return Quota{(positions - few * (kStreams / 2) + kStreams / 2 - 1) / (kStreams / 2), few};
