@@ -101,6 +101,8 @@ int32_t slots_call(const TensorCallV1* call, TensorErrorV1* error) {
   if (a[6].scalar >> 31 || !a[6].scalar) return fail(error, TENSOR_ERROR_ARGUMENT, "T: must be a positive int32");
   int64_t tokens[1] = {(int64_t)a[6].scalar}, one[1] = {1}, requests[1] = {-1}, free[1] = {-1}, table[2] = {-1, -1};
   CHECK(check_ints(a[0], "lengths", ordinal, requests, 1, error));
+  if (requests[0] * tensor_paged::kSlotsThreads > tensor_paged::kMostThreads)
+    return fail(error, TENSOR_ERROR_ARGUMENT, "lengths: less than 2^24 requests");
   table[0] = requests[0];
   int64_t ends[1] = {requests[0] + 1};
   CHECK(check_ints(a[1], "counts", ordinal, requests, 1, error));
@@ -191,6 +193,12 @@ int32_t rotary_call(const TensorCallV1* call, TensorErrorV1* error, bool store) 
     CHECK(check_apart(call, {{4, "q_out", 0}, {5, "k_out", 1}}, error));
     args.k_out = pointer<void>(a[5]);
   }
+  args.heads = (int)q[1];
+  args.kv = (int)k[1];
+  args.dim = (int)q[2];
+  args.rotated = (int)table[1];
+  if (q[0] * tensor_paged::rotary_threads(args) > tensor_paged::kMostThreads)
+    return fail(error, TENSOR_ERROR_ARGUMENT, "q: too many tokens for one call");
   CHECK(check_device(call, error));
   args.q = pointer<const void>(a[0]);
   args.k = pointer<const void>(a[1]);
@@ -198,10 +206,6 @@ int32_t rotary_call(const TensorCallV1* call, TensorErrorV1* error, bool store) 
   args.angles = pointer<const float>(angles);
   args.q_out = pointer<void>(q_out);
   args.tokens = (int)q[0];
-  args.heads = (int)q[1];
-  args.kv = (int)k[1];
-  args.dim = (int)q[2];
-  args.rotated = (int)table[1];
   args.reach = (int)table[0];
   args.interleaved = layout == 1;
   args.inverse = inverse == 1;
@@ -219,8 +223,9 @@ int32_t check_attention(int64_t tokens, int64_t requests, int64_t heads, int64_t
                 tensor_paged::kAttentionMaxShare);
   if (requests < 1 || requests > tensor_paged::kAttentionMaxRequests)
     return fail(error, TENSOR_ERROR_ARGUMENT, "1 to %d requests", tensor_paged::kAttentionMaxRequests);
-  if (tokens < 1 || tokens > 1 << 20 || tokens * heads >= (int64_t)1 << 31)
-    return fail(error, TENSOR_ERROR_ARGUMENT, "q: 1 to 2^20 tokens, less than 2^31 rows of heads");
+  // (the joining kernel has a thread for four values, in workgroups of up to 512)
+  if (tokens < 1 || tokens > 1 << 20 || tokens * heads * (dim / 4) > tensor_paged::kMostThreads - 512)
+    return fail(error, TENSOR_ERROR_ARGUMENT, "q: 1 to 2^20 tokens, less than 2^34 - 2048 values");
   return TENSOR_OK;
 }
 

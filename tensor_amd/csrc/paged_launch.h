@@ -13,6 +13,9 @@ struct SlotsArgs {
   int32_t *offsets, *lengths_out, *positions, *slots, *table_out, *free_left;
   int requests, columns, tokens, free_extent, page_shift;
 };
+// A launch has at most 2^32 - 1 threads along x.
+constexpr int64_t kMostThreads = ((int64_t)1 << 32) - 1;
+constexpr int kSlotsThreads = 256;  // of a request
 hipError_t launch_slots(const SlotsArgs& args, hipStream_t stream);
 
 struct RotaryArgs {
@@ -23,6 +26,7 @@ struct RotaryArgs {
   int tokens, heads, kv, dim, rotated, reach, pages, page_shift;
   bool interleaved, inverse, in_f32, out_f32;
 };
+int rotary_threads(const RotaryArgs& args);  // of a token's workgroup
 hipError_t launch_rotary(const RotaryArgs& args, hipStream_t stream);
 
 struct AttentionArgs {

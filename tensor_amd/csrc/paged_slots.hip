@@ -16,7 +16,7 @@
 namespace tensor_paged {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = kSlotsThreads;
 
 // Sums past int32 stop at its ends: a wrapped length would be none, a wrapped position padding.
 __device__ __forceinline__ int saturated(int64_t v) { return (int)max(min(v, (int64_t)INT32_MAX), (int64_t)INT32_MIN); }

@@ -142,14 +142,16 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a, int uni
   }
 }
 
+bool in_vectors(const RotaryArgs& a) { return a.dim % 16 == 0 && a.rotated % 16 == 0; }
+int units_of(const RotaryArgs& a) { return in_vectors(a) ? a.dim / 16 : a.dim - a.rotated / 2; }
+int64_t work_of(const RotaryArgs& a) { return (int64_t)units_of(a) * (a.heads + a.kv + (a.v ? a.kv : 0)); }
+
 template <typename In, typename Out>
 hipError_t launch_typed(const RotaryArgs& a, hipStream_t stream) {
-  const bool vector = a.dim % 16 == 0 && a.rotated % 16 == 0;
-  const int units = vector ? a.dim / 16 : a.dim - a.rotated / 2;
-  const int64_t work = (int64_t)units * (a.heads + a.kv + (a.v ? a.kv : 0));
-  const int64_t shares = (work + 255) / 256;
-  if (shares > 65535) return hipErrorInvalidValue;
-  const int threads = (int)((work + shares - 1) / shares + 63) / 64 * 64;  // whole waves, even shares
+  const bool vector = in_vectors(a);
+  const int units = units_of(a), threads = rotary_threads(a);
+  const int64_t work = work_of(a);
+  if ((work + 255) / 256 > 65535) return hipErrorInvalidValue;
   const dim3 grid(a.tokens, (unsigned)((work + threads - 1) / threads));
 #define LAUNCH(I, V) \
   hipLaunchKernelGGL((rotary_kernel<In, Out, I, V>), grid, dim3(threads), 0, stream, a, units, threads)
@@ -163,6 +165,11 @@ hipError_t launch_typed(const RotaryArgs& a, hipStream_t stream) {
 }
 
 }  // namespace
+
+int rotary_threads(const RotaryArgs& a) {
+  const int64_t work = work_of(a), shares = (work + 255) / 256;
+  return (int)((work + shares - 1) / shares + 63) / 64 * 64;  // whole waves, even shares
+}
 
 hipError_t launch_rotary(const RotaryArgs& a, hipStream_t stream) {
   if (a.in_f32) return a.out_f32 ? launch_typed<float, float>(a, stream) : launch_typed<float, _Float16>(a, stream);
