@@ -1,7 +1,7 @@
 /*
  * libtensor_hip.so — the ROCm (gfx950) provider's C ABI.
  *
- * Three groups of entry points:
+ * Four groups of entry points:
  *
  *  1. GGUF quantized-linear kernels, in the reference's native entry shape
  *     TensorKernelV1 (src/tensor/include/tensor/abi.h:135-141).  Each validates
@@ -18,7 +18,9 @@
  *
  *  2. The paged-cache operators (slot maps, rotary positions, attention), in the same shape.
  *
- *  3. Runtime services the Python provider binds through ctypes, replacing the
+ *  3. Norms and linears on 8-bit values with block scales, in the same shape.
+ *
+ *  4. Runtime services the Python provider binds through ctypes, replacing the
  *     CUDA driver calls of src/tensor/providers/cuda/driver.py:40-145
  *     (memory, copies, streams, events, graphs, device properties).
  *
@@ -353,6 +355,54 @@ int32_t tensor_paged_attention_v1(const TensorCallV1 *call, TensorErrorV1 *error
 /* Bytes of workspace tensor_paged_attention_v1 needs for these extents. */
 int32_t tensor_paged_attention_workspace_v1(int64_t tokens, int64_t requests, int64_t heads, int64_t kv_heads,
                                             int64_t dim, uint64_t *bytes, TensorErrorV1 *error);
+
+/* ------------------------------------ norms and 8-bit linears ---
+ *
+ * What a decoder layer runs around its attention when its linears are held in 8 bits.  No counterpart in the
+ * reference.  8 bits are e4m3 (a sign, four bits of exponent with bias 7, three of fraction; no infinities, NaN at 0x7F and
+ * 0xFF, values up to 448), in uint8 buffers.  A row of activations has a scale for each 128 columns,
+ * s = max(a / 448, 2^-126) with a the largest finite magnitude among them, and the codes nearest to value / s (ties to
+ * even; a value that is not finite has the NaN code).  Scales are held [blocks, rows], blocks = ceil(columns / 128).  Rows of
+ * weights have one for each block of 128 rows x 128 columns.  Buffers are contiguous and 16-byte aligned.  A
+ * call refuses a buffer that it writes and that shares memory with another of its buffers, except where it says that the two
+ * may be one.
+ */
+
+/*
+ * Root-mean-square norm of rows: h = x + residual, residual_out = h, out = h / sqrt(mean(h^2) + eps) * weight, in fp32, out
+ * and residual_out each rounded once from there.  Without a residual (four arguments) h = x.  Rows of up to 32768 values.
+ *    0 x            fp16 or fp32 [rows, width]
+ *    1 residual     fp16 or fp32 [rows, width]      (left out with residual_out)
+ *    2 weight       fp32 [width]
+ *    3 out          fp16 or fp32 [rows, width]      (may be x, of the same type)
+ *    4 residual_out as residual                     (may be residual)
+ *    5 eps          scalar fp32, positive
+ */
+int32_t tensor_rms_norm_v1(const TensorCallV1 *call, TensorErrorV1 *error);
+
+/*
+ * tensor_rms_norm_v1 with its result in 8 bits: [x, (residual,) weight, codes, scales, (residual_out,) eps], codes uint8
+ * [rows, width], scales fp32 [blocks, rows].
+ */
+int32_t tensor_rms_norm_fp8_v1(const TensorCallV1 *call, TensorErrorV1 *error);
+
+/*
+ * Rows in 8 bits: of x, or (gated = 1) of silu(g) * u for rows that hold width gates g, then width values u, silu(g) =
+ * g / (1 + exp(-g)), in fp32.
+ *    0 x      fp16 or fp32 [rows, width], gated [rows, 2 width]
+ *    1 codes  uint8 [rows, width]        2 scales fp32 [blocks, rows]        3 gated scalar uint32, 0 or 1
+ */
+int32_t tensor_quantize_fp8_v1(const TensorCallV1 *call, TensorErrorV1 *error);
+
+/*
+ * Linear layer on 8-bit operands: out[m, n] = sum_b (x_scales[b, m] w_scales[n / 128, b]) sum_{k in block b} x[m, k] w[n, k].
+ * The inner sums are the matrix cores', the outer one is kept in fp32; one rounding to the output's type.  The product of two
+ * scales is taken in fp32: below 2^-126 it loses bits, past fp32's largest the output is not finite.
+ *    0 x        uint8 [M, K], K a multiple of 16      1 x_scales fp32 [ceil(K / 128), M]
+ *    2 w        uint8 [N, K]                          3 w_scales fp32 [ceil(N / 128), ceil(K / 128)]
+ *    4 out      fp16 or fp32 [M, N]
+ */
+int32_t tensor_fp8_linear_v1(const TensorCallV1 *call, TensorErrorV1 *error);
 
 /* ---------------------------------------------------- runtime services --- */
 

@@ -33,6 +33,10 @@ KERNELS = (
     "tensor_rotary_v1",
     "tensor_rotary_store_v1",
     "tensor_paged_attention_v1",
+    "tensor_rms_norm_v1",
+    "tensor_rms_norm_fp8_v1",
+    "tensor_quantize_fp8_v1",
+    "tensor_fp8_linear_v1",
 )
 
 _u64, _i32, _f32p = c.c_uint64, c.c_int32, c.POINTER(c.c_float)

@@ -39,12 +39,13 @@ def _scalar(name: str, dtype: str = "uint32") -> dict:
     return {"name": name, "dtype": dtype, "kind": "scalar"}
 
 
-def _result(kernel: str, label: str, arguments: list, outputs: list, symbols: str, constants: dict, **more) -> dict:
+def _result(kernel: str, label: str, arguments: list, outputs: list, symbols: str, constants: dict, *,
+            entrypoint: str | None = None, **more) -> dict:
     return {
         "name": f"{kernel}:{label}",
         "provider": "hip",
         "target": "gfx950",
-        "entrypoint": ENTRYPOINTS[kernel],
+        "entrypoint": entrypoint or ENTRYPOINTS[kernel],
         "runtime_abi": {"major": 1, "minor": 1, "required_capabilities": [
             "contiguous", "executable_descriptors", "no_external_workspace", "scalars"]},
         "arguments": arguments,
