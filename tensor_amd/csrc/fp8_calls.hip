@@ -137,6 +137,7 @@ int32_t linear_call(const TensorCallV1* call, TensorErrorV1* error) {
   CHECK(check_values(a[4], "out", ordinal, out, 2, error));
   if (x[0] > 1 << 20 || w[0] > 1 << 22 || x[1] > 1 << 20)
     return fail(error, TENSOR_ERROR_ARGUMENT, "x, w: at most 2^20 rows of x, 2^22 of w, and 2^20 columns");
+  if (x[0] * w[0] > (int64_t)1 << 35) return fail(error, TENSOR_ERROR_ARGUMENT, "out: at most 2^35 values");
   CHECK(check_apart(call, {{4, "out", -1}}, error));
   CHECK(check_device(call, error));
   tensor_fp8::LinearArgs args{};

@@ -1,12 +1,17 @@
 // Linear layer on 8-bit operands with a scale for each block of 128 (fp8_common.h):
 //   out[m, n] = sum_b (sx[b, m] sw[n / 128, b]) sum_{k in block b} x[m, k] w[n, k]
-// The inner sum is the matrix cores', on operands widened to fp16, the outer one fp32 vector arithmetic on its results.
+// The inner sum is the matrix cores', the outer one fp32 vector arithmetic on its results.
+#include <type_traits>
+#include <utility>
+
 #include "fp8_common.h"
 
 namespace tensor_fp8 {
 namespace {
 
 typedef int int8v_t __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // 8 codes as the fp16 values that they stand for (exactly; NaN stays NaN)
 __device__ __forceinline__ half8_t widened(int lo, int hi) {
@@ -21,54 +26,393 @@ __device__ __forceinline__ half8_t widened(int lo, int hi) {
   return v;
 }
 
-// 16 weight rows x 16 activation rows: lane l has column l % 16 and rows 4 (l / 16) ..
-__device__ __forceinline__ float4_t products(int8v_t w, int8v_t x) {
+// An operand of 16 rows x 128 columns as the matrix instructions take it, lane l 32 columns of row l % 16 (any order
+// does that both operands share).
+struct Codes8 {
+  int8v_t v;
+  __device__ __forceinline__ void set(uint4 a, uint4 b) {
+    v = int8v_t{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+  }
+};
+struct Codes16 {
+  half8_t v[4];
+  __device__ __forceinline__ void set(uint4 a, uint4 b) {
+    v[0] = widened(a.x, a.y); v[1] = widened(a.z, a.w); v[2] = widened(b.x, b.y); v[3] = widened(b.z, b.w);
+  }
+};
+// 16 weight rows x 16 activation rows over 128 columns: lane l has activation row l % 16 and weight rows 4 (l / 16) ..
+__device__ __forceinline__ float4_t products(const Codes8& w, const Codes8& x) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, float4_t{}, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ float4_t products(const Codes16& w, const Codes16& x) {
   float4_t sum = {};
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(widened(w[2 * i], w[2 * i + 1]), widened(x[2 * i], x[2 * i + 1]), sum, 0, 0, 0);
+  for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[i], x.v[i], sum, 0, 0, 0);
   return sum;
 }
 
-// This lane's 32 bytes of a row's 128 columns from k on: chunks of 16 at l / 16 and 4 + l / 16 (any order does that
-// both operands share), zeros past the row's end.
-__device__ __forceinline__ int8v_t fragment(const uint8_t* row, int k, int columns, int lane) {
-  uint4 v[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int at = k + 16 * (4 * i + (lane >> 4));
-    v[i] = at < columns ? *reinterpret_cast<const uint4*>(row + at) : uint4{};
-  }
-  return int8v_t{(int)v[0].x, (int)v[0].y, (int)v[0].z, (int)v[0].w, (int)v[1].x, (int)v[1].y, (int)v[1].z, (int)v[1].w};
+typedef const float __attribute__((address_space(4))) Constant;  // loaded through the scalar cache
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(const void __attribute__((address_space(3)))*)p;
+}
+// 16 (or 4) bytes a lane from global memory to LDS, lane l to dst + 16 l (4 l); dst is the same in the whole wave.
+// Written as assembly: the compiler would make every LDS read wait for all such loads in flight; the waits are
+// written out where a stage is read.  (Nothing else here uses m0.)
+__device__ __forceinline__ void dma16(const void* base, uint32_t offset, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void dma4(const void* base, uint32_t offset, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory");
 }
 
-template <typename Out>
-__global__ __launch_bounds__(256) void linear_kernel(const LinearArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n0 = (blockIdx.x * 4 + wave) * 16, m0 = blockIdx.y * 16;
-  if (n0 >= a.n) return;
-  const int m = min(m0 + (lane & 15), a.m - 1), n = min(n0 + (lane & 15), a.n - 1), blocks = (a.k + kBlock - 1) / kBlock;
-  const uint8_t *x = a.x + (size_t)m * a.k, *w = a.w + (size_t)n * a.k;
-  float4_t sum = {};
-  for (int b = 0; b < blocks; ++b) {
-    const float scale = a.x_scales[(size_t)b * a.m + m] * a.w_scales[(size_t)(n0 / kBlock) * blocks + b];
-    sum += products(fragment(w, b * kBlock, a.k, lane), fragment(x, b * kBlock, a.k, lane)) * scale;
+constexpr int least(int a, int b) { return a < b ? a : b; }
+
+// f(0), f(1), .. f(N - 1), each with its number as a constant
+template <typename F, int... I>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& f) {
+  each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+// The order of a step's products in a wave of TN groups of 16 weight rows and TM of activation rows: the first half of
+// the groups one after another, then the second half by activation rows, and where a group is held meanwhile.
+template <int TN, int TM>
+struct Units {
+  static constexpr int COUNT = TN * TM, HALF = TN / 2;
+  static_assert(TN == 8 || TN == 4 || TN == 2, "the places of weight groups");
+  static constexpr int SLOTS = TN == 8 ? 5 : TN;
+  static constexpr int EARLY = TN == 2 ? 1 : 2;  // groups read before the step
+  static constexpr int group(int u) { return u < HALF * TM ? u / TM : HALF + (u - HALF * TM) % HALF; }
+  static constexpr int row(int u) { return u < HALF * TM ? u % TM : (u - HALF * TM) / HALF; }
+  static constexpr int slot(int i) { return TN == 8 && i < 6 ? (i % 3 ? i % 3 - 1 : 4) : TN == 8 ? i - 4 : i; }  // 4 0 1 4 0 1 2 3
+  // the group read beside product u (TN and on: the next step's), -1 for none
+  static constexpr int reads(int u) {
+    if (TN == 2) return u == 0 ? 1 : -1;
+    if (TN == 4) return u == 0 ? 2 : u == (TM + 1) / 2 ? 3 : -1;
+    return u == 0 ? 2 : u == TM / 2 ? 6 : u == TM ? 3 : u == TM + TM / 2 ? 7 : u == 2 * TM ? 4 : u == 3 * TM ? 5
+         : u == COUNT - HALF ? TN + 1 : -1;
   }
-  if (m0 + (lane & 15) >= a.m) return;
+};
+
+// A tile of BN weight rows x BM activation rows by WN x WM waves, K in steps of a block through STAGES places of LDS.
+template <typename Out, typename Codes, int BN, int BM, int WN, int WM, int STAGES>
+__global__ __launch_bounds__(64 * WN * WM, 2) void linear_tiles(const LinearArgs a, int tiles_n, int tiles_m) {
+  constexpr int NW = WN * WM, TN = BN / WN / 16, TM = BM / WM / 16;
+  constexpr int PW = BN / 8 / NW, PX = BM / 8 / NW;            // loads of a wave and step: 8 rows of 128 bytes each
+  constexpr int SCALES = BM < 64 ? 64 : BM;
+  constexpr int STAGE = (BN + BM) * 128 + 4 * SCALES;
+  static_assert(PW * 8 * NW == BN && PX * 8 * NW == BM, "whole loads for each wave");
+  static_assert(BN / WN <= 128, "a wave's weight rows share a scale");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * STAGE];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), quad = lane >> 4;
+
+  // Workgroups go round the eight XCDs in turn: each XCD has a range of the tiles, eight of x by all of w at a time.
+  const int total = tiles_n * tiles_m, share = (total + 7) / 8;
+  const int index = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= share || index >= total) return;
+  constexpr int GROUP = 8;
+  const int group = index / (GROUP * tiles_n), first = group * GROUP, deep = min(GROUP, tiles_m - first);
+  const int within = index - group * GROUP * tiles_n;
+  const int n0 = within / deep * BN, m0 = (first + within % deep) * BM;
+
+  const int steps = (a.k + kBlock - 1) / kBlock;
+  const uint32_t lds_at = lds_address(lds);
+  // this lane's source of each load: its row of 8, its chunk swizzled by the row, which is where LDS reads look for it
+  const int chunk = (lane & 7) ^ (lane >> 3);
+  const int part = 64 * (wave % (SCALES / 64));
+  const uint32_t s_at = 4 * min(part + lane, a.m - 1 - m0);
+  const uint8_t* const w = a.w + (size_t)n0 * a.k;
+  const uint8_t* const x = a.x + (size_t)m0 * a.k;
+  // Part p of stage t: a load of weights, of activations, of their scales.  (A lane's offset is worked out each time:
+  // registers are what a wave has least of.)
+  constexpr int PARTS = PW + PX + 1;
+  auto load = [&](int t, int p) {
+    const uint32_t to = lds_at + (t % STAGES) * STAGE;
+    const int k = t * kBlock;
+    if (p == PW + PX) {
+      dma4(a.x_scales + (size_t)t * a.m + m0, s_at, to + 128 * (BN + BM) + 4 * part);
+      return;
+    }
+    const bool weights = p < PW;
+    const int rows = 8 * (weights ? wave * PW + p : wave * PX + p - PW);
+    int r = lane >> 3;
+    asm volatile("" : "+v"(r));
+    const int column = min(16 * chunk, a.k - k - 16);  // past the row's end: its last chunk (cleared below)
+    const uint32_t at = __umul24(min(rows + r, (weights ? a.n - n0 : a.m - m0) - 1), a.k) + column;
+    dma16((weights ? w : x) + k, at, to + 128 * rows + (weights ? 0 : 128 * BN));
+  };
+  auto load_all = [&](int t) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int at = n0 + 4 * (lane >> 4) + e;
-    if (at < a.n) static_cast<Out*>(a.out)[(size_t)m * a.n + at] = (Out)sum[e];
+    for (int p = 0; p < PARTS; ++p) load(t, p);
+  };
+  // Columns past the row's end in the last stage are zeros: this wave's part of it, when it has landed.
+  auto clear_past = [&](int t) {
+    if (t * kBlock + 16 * chunk < a.k) return;
+#pragma unroll
+    for (int j = 0; j < PW + PX; ++j) {
+      const int at = j < PW ? 1024 * (wave * PW + j) : 128 * BN + 1024 * (wave * PX + j - PW);
+      *reinterpret_cast<uint4*>(lds + (t % STAGES) * STAGE + at + 16 * lane) = uint4{};
+    }
+  };
+
+  const int wn = wave % WN, wm = wave / WN;
+  const Constant* const w_scale = (const Constant*)(uintptr_t)a.w_scales + (size_t)min((n0 + wn * 16 * TN) / kBlock, (a.n - 1) / kBlock) * steps;
+  float4_t acc[TN][TM] = {};
+  // this lane's chunks of row r of a staged matrix
+  auto read = [&](Codes& to, const uint8_t* matrix, int row) {
+    const int r = row + (lane & 15);
+    to.set(*reinterpret_cast<const uint4*>(matrix + 128 * r + 16 * (quad ^ (r & 7))),
+           *reinterpret_cast<const uint4*>(matrix + 128 * r + 16 * ((4 + quad) ^ (r & 7))));
+  };
+  // Products one after another, each followed by the scaled sum of the one DEEP - 1 before it, whose result is there by
+  // then.  The first half of the wave's weight groups goes by groups; by its end all of the second half is in registers,
+  // the next stage takes this one's place, and the second half goes by activation rows, each of which makes
+  // room for the next step's: LDS reads are spread over the step.
+  constexpr int DEEP = 3, HALF = TN / 2, APART = BN == 256 ? 7 : 0;
+  using Order = Units<TN, TM>;
+  constexpr int UNITS = Order::COUNT;
+  Codes xs[TM], ws[Order::SLOTS];
+  float scale[TM], next_scale[TM];
+  float4_t sums[DEEP];
+  auto place = [&](int t) { return lds + (t % STAGES) * STAGE; };
+  auto read_w = [&](int t, int i) { read(ws[Order::slot(i)], place(t), wn * 16 * TN + 16 * i); };
+  auto read_x = [&](int t, int j) {
+    read(xs[j], place(t) + 128 * BN, wm * 16 * TM + 16 * j);
+    next_scale[j] = reinterpret_cast<const float*>(place(t) + 128 * (BN + BM))[wm * 16 * TM + 16 * j + (lane & 15)];
+  };
+  // Waits until stage t has landed, this wave's part and after the barrier everyone's.
+  auto landed = [&](int t, int issued) {
+    if (STAGES > 2 && issued < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * PARTS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (t + 1 == steps) clear_past(t);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+  each<STAGES - 1>([&](auto t) { if (t < steps) load_all(t); });
+  landed(0, STAGES - 2);
+  if (STAGES - 1 < steps) load_all(STAGES - 1);
+  each<Order::EARLY>([&](auto i) { read_w(0, i); });
+  each<TM>([&](auto j) { read_x(0, j); });
+  float sw = w_scale[0];
+  for (int t = 0; t < steps; ++t) {
+    float next_sw = w_scale[min(t + 1, steps - 1)];
+    each<TM>([&](auto j) { scale[j] = next_scale[j] * sw; });
+    each<UNITS + DEEP - 1>([&](auto unit) {
+      constexpr int u = decltype(unit)::value;
+      if constexpr (u == HALF * TM) {
+        landed(t + 1, t + STAGES - 1);  // (nobody reads stage t any more)
+        asm volatile("" : "+s"(next_sw));
+        read_w(t + 1, 0);
+        if constexpr (TN == 4) read_w(t + 1, 1);
+      }
+      if constexpr (u < UNITS) {
+        constexpr int i = Order::group(u), j = Order::row(u);
+        if constexpr (u >= HALF * TM) {
+          if (t + STAGES < steps)
+            each<PARTS>([&](auto p) {
+              if constexpr (least(decltype(p)::value * APART / 4, UNITS - HALF * TM - 1) == u - HALF * TM) load(t + STAGES, p);
+            });
+        }
+        sums[u % DEEP] = products(ws[Order::slot(i)], xs[j]);
+        if constexpr (Order::reads(u) >= 0) read_w(t + Order::reads(u) / TN, Order::reads(u) % TN);
+        if constexpr (i == TN - 1) read_x(t + 1, j);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (u >= DEEP - 1) {
+        constexpr int v = u - DEEP + 1, i = Order::group(v), j = Order::row(v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] += sums[v % DEEP][e] * scale[j];
+        asm volatile("" : "+v"(acc[i][j]));  // made here, not where it is used
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    sw = next_sw;
+  }
+  // 16 activation rows at a time through LDS, a place for each wave (of the stage that nobody reads: `steps`), so
+  // that stores are of 16 bytes a lane and whole lines.
+  constexpr int COLUMNS = 16 * TN, PER = 16 / sizeof(Out), ROW = COLUMNS + PER;  // (rows shifted by four banks each)
+  static_assert(NW * 16 * ROW * sizeof(Out) <= STAGE, "a wave's place");
+  typedef Out Out4 __attribute__((ext_vector_type(4)));
+  typedef Out Chunk __attribute__((ext_vector_type(PER)));
+  Out* const mine = reinterpret_cast<Out*>(lds + (steps % STAGES) * STAGE) + wave * 16 * ROW;
+#pragma unroll
+  for (int j = 0; j < TM; ++j) {
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+      *reinterpret_cast<Out4*>(mine + (lane & 15) * ROW + 16 * i + 4 * quad) = __builtin_convertvector(acc[i][j], Out4);
+#pragma unroll
+    for (int r = 0; r < 16 * COLUMNS / PER / 64; ++r) {
+      const int at = 64 * r + lane, row = at / (COLUMNS / PER), column = at % (COLUMNS / PER) * PER;
+      const Chunk v = *reinterpret_cast<const Chunk*>(mine + row * ROW + column);
+      const int m = m0 + wm * 16 * TM + 16 * j + row, n = n0 + wn * 16 * TN + column;
+      if (m >= a.m || n >= a.n) continue;
+      Out* const to = static_cast<Out*>(a.out) + (size_t)m * a.n + n;
+      if (n + PER <= a.n) {
+        __builtin_memcpy(to, &v, sizeof(v));
+      } else {
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          if (n + e < a.n) to[e] = v[e];
+      }
+    }
+  }
+}
+
+// Few activation rows (decode): 16 GN weight rows x 16 GM activation rows (of which XR are staged) by WAVES waves, each of
+// which streams its own steps of K through STAGES places of its own in LDS, without barriers; their sums meet at the end.
+template <typename Out, typename Codes, int GN, int GM, int XR, int WAVES, int STAGES>
+__global__ __launch_bounds__(64 * WAVES) void linear_rows(const LinearArgs a, int tiles_m) {
+  constexpr int BN = 16 * GN, BM = 16 * GM, PW = BN / 8, PX = XR / 8, PARTS = PW + PX + 1;
+  constexpr int STAGE = (BN + XR) * 128 + 256;
+  constexpr int SUMS = 4 * BN * BM;
+  static_assert(SUMS <= STAGES * STAGE && XR <= BM, "a wave's sums");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[WAVES * STAGES * STAGE];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), quad = lane >> 4;
+  // workgroups go round the eight XCDs in turn: those of the same weight rows are neighbours on one of them
+  const int tile = blockIdx.x >> 3, n0 = ((tile / tiles_m) * 8 + (blockIdx.x & 7)) * BN, m0 = tile % tiles_m * XR;
+  if (n0 >= a.n) return;
+  const int steps = (a.k + kBlock - 1) / kBlock, mine = (steps - wave + WAVES - 1) / WAVES;
+  uint8_t* const ring = lds + wave * STAGES * STAGE;
+  const uint32_t ring_at = lds_address(ring);
+  const int chunk = (lane & 7) ^ (lane >> 3);
+  const uint8_t* const w = a.w + (size_t)n0 * a.k;
+  const uint8_t* const x = a.x + (size_t)m0 * a.k;
+  uint32_t w_at[PW], x_at[PX];
+#pragma unroll
+  for (int p = 0; p < PW; ++p) w_at[p] = __umul24(min(8 * p + (lane >> 3), a.n - 1 - n0), a.k);
+#pragma unroll
+  for (int p = 0; p < PX; ++p) x_at[p] = __umul24(min(8 * p + (lane >> 3), a.m - 1 - m0), a.k);
+  const uint32_t s_at = 4 * min(min(lane, XR - 1), a.m - 1 - m0);
+  auto load = [&](int i) {
+    const int b = wave + i * WAVES, k = b * kBlock;
+    const uint32_t to = ring_at + (i % STAGES) * STAGE;
+    const int column = min(16 * chunk, a.k - k - 16);  // past the row's end: its last chunk (cleared below)
+#pragma unroll
+    for (int p = 0; p < PW; ++p) dma16(w + k, w_at[p] + column, to + 1024 * p);
+#pragma unroll
+    for (int p = 0; p < PX; ++p) dma16(x + k, x_at[p] + column, to + 128 * BN + 1024 * p);
+    dma4(a.x_scales + (size_t)b * a.m + m0, s_at, to + 128 * (BN + XR));
+  };
+  auto read = [&](Codes& to, const uint8_t* matrix, int r) {
+    to.set(*reinterpret_cast<const uint4*>(matrix + 128 * r + 16 * (quad ^ (r & 7))),
+           *reinterpret_cast<const uint4*>(matrix + 128 * r + 16 * ((4 + quad) ^ (r & 7))));
+  };
+  const Constant* const w_scale = (const Constant*)(uintptr_t)a.w_scales + (size_t)(n0 / kBlock) * steps;
+  float4_t acc[GN][GM] = {};
+  each<STAGES - 1>([&](auto i) { if (i < mine) load(i); });
+  for (int i = 0; i < mine; ++i) {
+    const int b = wave + i * WAVES;
+    const float sw = w_scale[b];
+    if (i + STAGES - 2 < mine) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * PARTS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    uint8_t* const at = ring + (i % STAGES) * STAGE;
+    if ((b + 1) * kBlock > a.k && b * kBlock + 16 * chunk >= a.k) {  // columns past the row's end are zeros
+#pragma unroll
+      for (int p = 0; p < PW + PX; ++p) *reinterpret_cast<uint4*>(at + 1024 * p + 16 * lane) = uint4{};
+    }
+    Codes ws[GN], xs[GM];
+    float scale[GM];
+#pragma unroll
+    for (int g = 0; g < GN; ++g) read(ws[g], at, 16 * g + (lane & 15));
+#pragma unroll
+    for (int g = 0; g < GM; ++g) {
+      read(xs[g], at + 128 * BN, (16 * g + (lane & 15)) % XR);
+      scale[g] = reinterpret_cast<const float*>(at + 128 * (BN + XR))[16 * g + (lane & 15)] * sw;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage before this one has been read too
+    if (i + STAGES - 1 < mine) load(i + STAGES - 1);
+#pragma unroll
+    for (int g = 0; g < GN; ++g)
+#pragma unroll
+      for (int j = 0; j < GM; ++j) acc[g][j] += products(ws[g], xs[j]) * scale[j];
+  }
+  // each wave's sums, in place of its stages; every thread adds up some outputs over the waves
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  float* const sums = reinterpret_cast<float*>(ring);
+#pragma unroll
+  for (int g = 0; g < GN; ++g)
+#pragma unroll
+    for (int j = 0; j < GM; ++j) *reinterpret_cast<float4_t*>(sums + (16 * j + (lane & 15)) * BN + 16 * g + 4 * quad) = acc[g][j];
+  __syncthreads();
+  for (int at = threadIdx.x; at < BN * BM; at += 64 * WAVES) {
+    const int m = m0 + at / BN, n = n0 + at % BN;
+    if (m >= a.m || n >= a.n || (XR < BM && at / BN >= XR)) continue;
+    float sum = 0.0f;
+#pragma unroll
+    for (int wv = 0; wv < WAVES; ++wv) sum += reinterpret_cast<const float*>(lds + wv * STAGES * STAGE)[at];
+    static_cast<Out*>(a.out)[(size_t)m * a.n + n] = (Out)sum;
+  }
+}
+
+template <typename Out, typename Codes, int GN, int GM, int XR, int WAVES, int STAGES>
+hipError_t launch_rows(const LinearArgs& a, hipStream_t stream) {
+  const int tiles_n = (a.n + 16 * GN - 1) / (16 * GN), tiles_m = (a.m + XR - 1) / XR;
+  hipLaunchKernelGGL((linear_rows<Out, Codes, GN, GM, XR, WAVES, STAGES>), dim3((tiles_n + 7) / 8 * 8 * tiles_m), dim3(64 * WAVES), 0,
+                     stream, a, tiles_m);
+  return hipGetLastError();
+}
+
+template <typename Out, typename Codes, int BN, int BM, int WN, int WM, int STAGES>
+hipError_t launch_tiles(const LinearArgs& a, hipStream_t stream) {
+  const int tiles_n = (a.n + BN - 1) / BN, tiles_m = (a.m + BM - 1) / BM;
+  const int64_t total = (int64_t)tiles_n * tiles_m;
+  hipLaunchKernelGGL((linear_tiles<Out, Codes, BN, BM, WN, WM, STAGES>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WN * WM), 0, stream, a, tiles_n, tiles_m);
+  return hipGetLastError();
+}
+
+// What a call would take in one of the kernels, in microseconds: workgroups go round the CUs, `beside` at a time on one of
+// them; a round costs `start` and a step of K `alone` with one workgroup on a CU, `full` with `beside`.  Figures of 32 to 128
+// steps, weights out of the caches (rows kernels: of M = 8, 16, 32 and 64; tiles: of M = 64 to 8192).
+struct Cost {
+  int bn, bm, beside;
+  float start, alone, full;
+  float of(const LinearArgs& a) const {
+    const int64_t groups = (int64_t)((a.n + bn - 1) / bn) * ((a.m + bm - 1) / bm), each_cu = (groups + 255) / 256;
+    if (groups > (int64_t)1 << 22) return 1e30f;  // (launches of up to 2^32 - 1 threads)
+    const int64_t rounds = each_cu / beside, rest = each_cu % beside;
+    const float steps = (float)blocks_of(a.k), part = beside > 1 ? (full - alone) / (beside - 1) : 0.0f;
+    const float round = start + steps * full;
+    return rounds * round + (rest ? start + steps * (alone + part * (rest - 1)) : 0.0f) - (beside == 1 && rounds == 1 ? steps * (full - alone) : 0.0f);
+  }
+};
+
+template <typename Out, typename Codes>
+hipError_t launch_typed(const LinearArgs& a, hipStream_t stream) {
+#ifdef PROBE_ROWS
+  return launch_rows<Out, Codes, PROBE_ROWS>(a, stream);
+#endif
+#ifdef PROBE_TILE
+  if constexpr (sizeof(Out) == 2) return launch_tiles<Out, Codes, PROBE_TILE>(a, stream);
+#endif
+  constexpr Cost rows16x8{16, 8, 2, 2.8f, 0.062f, 0.13f}, rows32x16{32, 16, 1, 2.8f, 0.10f, 0.13f}, rows16x32{16, 32, 1, 3.0f, 0.075f, 0.075f},
+      rows32x32{32, 32, 1, 3.0f, 0.11f, 0.17f}, tiles64{64, 64, 2, 2.3f, 0.33f, 0.42f}, tiles128x64{128, 64, 3, 2.8f, 0.55f, 0.85f},
+      tiles128{128, 128, 2, 1.8f, 0.69f, 1.13f}, tiles256{256, 256, 1, 5.0f, 1.32f, 1.72f};
+  const Cost* const costs[] = {&rows16x8, &rows32x16, &rows16x32, &rows32x32, &tiles64, &tiles128x64, &tiles128, &tiles256};
+  constexpr int count = sizeof(Out) == 2 ? 8 : 7;  // (256 x 256 tiles of widened operands do not fit the registers)
+  int best = 0;
+  for (int i = 1; i < count; ++i)
+    if (costs[i]->of(a) < costs[best]->of(a)) best = i;
+  switch (best) {
+    case 0: return launch_rows<Out, Codes, 1, 1, 8, 8, 3>(a, stream);
+    case 1: return launch_rows<Out, Codes, 2, 1, 16, 8, 3>(a, stream);
+    case 2: return launch_rows<Out, Codes, 1, 2, 32, 8, 3>(a, stream);
+    case 3: return launch_rows<Out, Codes, 2, 2, 32, 4, 3>(a, stream);
+    case 4: return launch_tiles<Out, Codes, 64, 64, 2, 2, 4>(a, stream);
+    case 5: return launch_tiles<Out, Codes, 128, 64, 2, 2, 2>(a, stream);
+    case 6: return launch_tiles<Out, Codes, 128, 128, 2, 2, 2>(a, stream);
+    default:
+      if constexpr (sizeof(Out) == 2) return launch_tiles<Out, Codes, 256, 256, 2, 4, 2>(a, stream);
+      return hipErrorInvalidValue;
   }
 }
 
 }  // namespace
 
 hipError_t launch_linear(const LinearArgs& a, hipStream_t stream) {
-  const dim3 grid((a.n + 63) / 64, (a.m + 15) / 16);
-  if (a.out_f32) hipLaunchKernelGGL((linear_kernel<float>), grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((linear_kernel<_Float16>), grid, dim3(256), 0, stream, a);
-  return hipGetLastError();
+  return a.out_f32 ? launch_typed<float, Codes16>(a, stream) : launch_typed<_Float16, Codes8>(a, stream);
 }
 
 }  // namespace tensor_fp8
