@@ -120,34 +120,43 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tiles(const LinearArgs
   const int n0 = within / deep * BN, m0 = (first + within % deep) * BM;
 
   const int steps = (a.k + kBlock - 1) / kBlock;
-  const uint32_t lds_at = lds_address(lds);
-  // this lane's source of each load: its row of 8, its chunk swizzled by the row, which is where LDS reads look for it
-  const int chunk = (lane & 7) ^ (lane >> 3);
-  const int part = 64 * (wave % (SCALES / 64));
-  const uint32_t s_at = 4 * min(part + lane, a.m - 1 - m0);
-  const uint8_t* const w = a.w + (size_t)n0 * a.k;
-  const uint8_t* const x = a.x + (size_t)m0 * a.k;
-  // Part p of stage t: a load of weights, of activations, of their scales.  (A lane's offset is worked out each time:
-  // registers are what a wave has least of.)
+  // This lane's source of each load: its row of 8, its chunk swizzled by the row, which is where LDS reads look for it.
+  // (256 x 256 tiles work it out each time: registers are what their waves have least of.)
+  constexpr bool HELD = BN * BM < 256 * 256;
   constexpr int PARTS = PW + PX + 1;
-  auto load = [&](int t, int p) {
-    const uint32_t to = lds_at + (t % STAGES) * STAGE;
-    const int k = t * kBlock;
+  const int chunk = (lane & 7) ^ (lane >> 3), rows_w = a.n - n0 - 1, rows_x = a.m - m0 - 1;
+  auto offset = [&](int p) {
+    int r = lane >> 3;
+    if (!HELD) asm volatile("" : "+v"(r));
+    return p < PW ? __umul24(min(8 * (wave * PW + p) + r, rows_w), a.k) + 16 * chunk
+                  : __umul24(min(8 * (wave * PX + p - PW) + r, rows_x), a.k) + 16 * chunk;
+  };
+  uint32_t held[HELD ? PARTS - 1 : 1];
+  if constexpr (HELD) each<PARTS - 1>([&](auto p) { held[p] = offset(p); });
+  const int part = 64 * (wave % (SCALES / 64));
+  const uint32_t s_at = 4 * min(part + lane, rows_x);
+  const uint32_t lds_w = lds_address(lds) + 1024 * wave * PW, lds_x = lds_address(lds) + 128 * BN + 1024 * wave * PX,
+                 lds_s = lds_address(lds) + 128 * (BN + BM) + 4 * part;
+  // The next stage to be loaded: its columns and its scales; `load` does part p of it, into place s (LAST: it may be
+  // the last one, whose columns past the row's end are read from its last chunk and cleared below).
+  const uint8_t *w = a.w + (size_t)n0 * a.k, *x = a.x + (size_t)m0 * a.k;
+  const float* x_scale = a.x_scales + m0;
+  auto load = [&](int t, auto s, int p, auto last) {
+    const int to = s * STAGE;
     if (p == PW + PX) {
-      dma4(a.x_scales + (size_t)t * a.m + m0, s_at, to + 128 * (BN + BM) + 4 * part);
+      dma4(x_scale, s_at, lds_s + to);
+      w += kBlock;
+      x += kBlock;
+      x_scale += a.m;
       return;
     }
-    const bool weights = p < PW;
-    const int rows = 8 * (weights ? wave * PW + p : wave * PX + p - PW);
-    int r = lane >> 3;
-    asm volatile("" : "+v"(r));
-    const int column = min(16 * chunk, a.k - k - 16);  // past the row's end: its last chunk (cleared below)
-    const uint32_t at = __umul24(min(rows + r, (weights ? a.n - n0 : a.m - m0) - 1), a.k) + column;
-    dma16((weights ? w : x) + k, at, to + 128 * rows + (weights ? 0 : 128 * BN));
+    uint32_t at = HELD ? held[HELD ? p : 0] : offset(p);
+    if (decltype(last)::value) at -= max(16 * chunk - (a.k - t * kBlock - 16), 0);
+    if (p < PW) dma16(w, at, lds_w + to + 1024 * p);
+    else dma16(x, at, lds_x + to + 1024 * (p - PW));
   };
-  auto load_all = [&](int t) {
-#pragma unroll
-    for (int p = 0; p < PARTS; ++p) load(t, p);
+  auto load_all = [&](int t, auto s) {
+    each<PARTS>([&](auto p) { load(t, s, p, std::true_type{}); });
   };
   // Columns past the row's end in the last stage are zeros: this wave's part of it, when it has landed.
   auto clear_past = [&](int t) {
@@ -160,14 +169,9 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tiles(const LinearArgs
   };
 
   const int wn = wave % WN, wm = wave / WN;
-  const Constant* const w_scale = (const Constant*)(uintptr_t)a.w_scales + (size_t)min((n0 + wn * 16 * TN) / kBlock, (a.n - 1) / kBlock) * steps;
+  // the present step's scale of the wave's weight rows
+  const Constant* w_scale = (const Constant*)(uintptr_t)a.w_scales + (size_t)min((n0 + wn * 16 * TN) / kBlock, (a.n - 1) / kBlock) * steps;
   float4_t acc[TN][TM] = {};
-  // this lane's chunks of row r of a staged matrix
-  auto read = [&](Codes& to, const uint8_t* matrix, int row) {
-    const int r = row + (lane & 15);
-    to.set(*reinterpret_cast<const uint4*>(matrix + 128 * r + 16 * (quad ^ (r & 7))),
-           *reinterpret_cast<const uint4*>(matrix + 128 * r + 16 * ((4 + quad) ^ (r & 7))));
-  };
   // Products one after another, each followed by the scaled sum of the one DEEP - 1 before it, whose result is there by
   // then.  The first half of the wave's weight groups goes by groups; by its end all of the second half is in registers,
   // the next stage takes this one's place, and the second half goes by activation rows, each of which makes
@@ -178,11 +182,17 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tiles(const LinearArgs
   Codes xs[TM], ws[Order::SLOTS];
   float scale[TM], next_scale[TM];
   float4_t sums[DEEP];
-  auto place = [&](int t) { return lds + (t % STAGES) * STAGE; };
-  auto read_w = [&](int t, int i) { read(ws[Order::slot(i)], place(t), wn * 16 * TN + 16 * i); };
-  auto read_x = [&](int t, int j) {
-    read(xs[j], place(t) + 128 * BN, wm * 16 * TM + 16 * j);
-    next_scale[j] = reinterpret_cast<const float*>(place(t) + 128 * (BN + BM))[wm * 16 * TM + 16 * j + (lane & 15)];
+  // this lane's two chunks of a staged row, of the wave's first weight and activation rows; its first scale
+  const int at0 = 128 * (lane & 15) + 16 * (quad ^ (lane & 7)), at1 = 128 * (lane & 15) + 16 * ((4 + quad) ^ (lane & 7));
+  const uint8_t *const w0 = lds + 2048 * wn * TN + at0, *const w1 = lds + 2048 * wn * TN + at1;
+  const uint8_t *const x0 = lds + 128 * BN + 2048 * wm * TM + at0, *const x1 = lds + 128 * BN + 2048 * wm * TM + at1;
+  const uint8_t* const s0 = lds + 128 * (BN + BM) + 4 * (16 * wm * TM + (lane & 15));
+  auto read_w = [&](auto s, int i) {
+    ws[Order::slot(i)].set(*reinterpret_cast<const uint4*>(w0 + s * STAGE + 2048 * i), *reinterpret_cast<const uint4*>(w1 + s * STAGE + 2048 * i));
+  };
+  auto read_x = [&](auto s, int j) {
+    xs[j].set(*reinterpret_cast<const uint4*>(x0 + s * STAGE + 2048 * j), *reinterpret_cast<const uint4*>(x1 + s * STAGE + 2048 * j));
+    next_scale[j] = *reinterpret_cast<const float*>(s0 + s * STAGE + 64 * j);
   };
   // Waits until stage t has landed, this wave's part and after the barrier everyone's.
   auto landed = [&](int t, int issued) {
@@ -191,34 +201,34 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tiles(const LinearArgs
     if (t + 1 == steps) clear_past(t);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
-  each<STAGES - 1>([&](auto t) { if (t < steps) load_all(t); });
-  landed(0, STAGES - 2);
-  if (STAGES - 1 < steps) load_all(STAGES - 1);
-  each<Order::EARLY>([&](auto i) { read_w(0, i); });
-  each<TM>([&](auto j) { read_x(0, j); });
-  float sw = w_scale[0];
-  for (int t = 0; t < steps; ++t) {
-    float next_sw = w_scale[min(t + 1, steps - 1)];
+  float sw = *w_scale;
+  // Step t, whose stage is in place s.  LAST: the steps from which on less than STAGES follow.
+  auto step = [&](int t, auto s, auto s_next, int ahead, auto last) {
+    constexpr bool LAST = decltype(last)::value;
+    float next_sw = w_scale[ahead];
     each<TM>([&](auto j) { scale[j] = next_scale[j] * sw; });
     each<UNITS + DEEP - 1>([&](auto unit) {
       constexpr int u = decltype(unit)::value;
-      if constexpr (u == HALF * TM) {
-        landed(t + 1, t + STAGES - 1);  // (nobody reads stage t any more)
+      if constexpr (u == HALF * TM) {  // (after the barrier nobody reads stage t any more)
+        if constexpr (LAST) landed(t + 1, t + STAGES - 1);
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * PARTS) : "memory");
         asm volatile("" : "+s"(next_sw));
-        read_w(t + 1, 0);
-        if constexpr (TN == 4) read_w(t + 1, 1);
+        read_w(s_next, 0);
+        if constexpr (TN == 4) read_w(s_next, 1);
       }
       if constexpr (u < UNITS) {
         constexpr int i = Order::group(u), j = Order::row(u);
         if constexpr (u >= HALF * TM) {
-          if (t + STAGES < steps)
+          if (!LAST || t + STAGES < steps)
             each<PARTS>([&](auto p) {
-              if constexpr (least(decltype(p)::value * APART / 4, UNITS - HALF * TM - 1) == u - HALF * TM) load(t + STAGES, p);
+              if constexpr (least(decltype(p)::value * APART / 4, UNITS - HALF * TM - 1) == u - HALF * TM) load(t + STAGES, s, p, last);
             });
         }
         sums[u % DEEP] = products(ws[Order::slot(i)], xs[j]);
-        if constexpr (Order::reads(u) >= 0) read_w(t + Order::reads(u) / TN, Order::reads(u) % TN);
-        if constexpr (i == TN - 1) read_x(t + 1, j);
+        constexpr int r = Order::reads(u);
+        if constexpr (r >= TN) read_w(s_next, r - TN);
+        else if constexpr (r >= 0) read_w(s, r);
+        if constexpr (i == TN - 1) read_x(s_next, j);
       }
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (u >= DEEP - 1) {
@@ -230,23 +240,42 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tiles(const LinearArgs
       __builtin_amdgcn_sched_barrier(0);
     });
     sw = next_sw;
+  };
+  each<STAGES - 1>([&](auto t) { if (t < steps) load_all(t, t); });
+  landed(0, STAGES - 2);
+  if (STAGES - 1 < steps) load_all(STAGES - 1, std::integral_constant<int, STAGES - 1>{});
+  constexpr std::integral_constant<int, 0> first_place{};
+  each<Order::EARLY>([&](auto i) { read_w(first_place, i); });
+  each<TM>([&](auto j) { read_x(first_place, j); });
+  int t = 0;
+  for (; HELD && t + 2 * STAGES <= steps - 1; t += STAGES) {
+    each<STAGES>([&](auto s) {
+      constexpr int next = (decltype(s)::value + 1) % STAGES;
+      step(t + s, s, std::integral_constant<int, next>{}, s + 1, std::false_type{});
+    });
+    w_scale += STAGES;
   }
-  // 16 activation rows at a time through LDS, a place for each wave (of the stage that nobody reads: `steps`), so
-  // that stores are of 16 bytes a lane and whole lines.
+#pragma unroll 1
+  for (; t < steps; ++t) {
+    step(t, t % STAGES, (t + 1) % STAGES, t + 1 < steps ? 1 : 0, std::true_type{});
+    ++w_scale;
+  }
+  // 16 activation rows at a time through LDS, a place for each wave, so that stores are of 16 bytes a lane and whole
+  // lines.  (Past the last step's barrier nobody needs what a stage holds.)
   constexpr int COLUMNS = 16 * TN, PER = 16 / sizeof(Out), ROW = COLUMNS + PER;  // (rows shifted by four banks each)
-  static_assert(NW * 16 * ROW * sizeof(Out) <= STAGE, "a wave's place");
+  static_assert(NW * 16 * ROW * sizeof(Out) <= STAGES * STAGE, "a wave's place");
   typedef Out Out4 __attribute__((ext_vector_type(4)));
   typedef Out Chunk __attribute__((ext_vector_type(PER)));
-  Out* const mine = reinterpret_cast<Out*>(lds + (steps % STAGES) * STAGE) + wave * 16 * ROW;
+  Out* const own = reinterpret_cast<Out*>(lds) + wave * 16 * ROW;
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
 #pragma unroll
     for (int i = 0; i < TN; ++i)
-      *reinterpret_cast<Out4*>(mine + (lane & 15) * ROW + 16 * i + 4 * quad) = __builtin_convertvector(acc[i][j], Out4);
+      *reinterpret_cast<Out4*>(own + (lane & 15) * ROW + 16 * i + 4 * quad) = __builtin_convertvector(acc[i][j], Out4);
 #pragma unroll
     for (int r = 0; r < 16 * COLUMNS / PER / 64; ++r) {
       const int at = 64 * r + lane, row = at / (COLUMNS / PER), column = at % (COLUMNS / PER) * PER;
-      const Chunk v = *reinterpret_cast<const Chunk*>(mine + row * ROW + column);
+      const Chunk v = *reinterpret_cast<const Chunk*>(own + row * ROW + column);
       const int m = m0 + wm * 16 * TM + 16 * j + row, n = n0 + wn * 16 * TN + column;
       if (m >= a.m || n >= a.n) continue;
       Out* const to = static_cast<Out*>(a.out) + (size_t)m * a.n + n;
@@ -364,18 +393,21 @@ hipError_t launch_tiles(const LinearArgs& a, hipStream_t stream) {
 }
 
 // What a call would take in one of the kernels, in microseconds: workgroups go round the CUs, `beside` at a time on one of
-// them; a round costs `start` and a step of K `alone` with one workgroup on a CU, `full` with `beside`.  Figures of 32 to 128
-// steps, weights out of the caches (rows kernels: of M = 8, 16, 32 and 64; tiles: of M = 64 to 8192).
+// them; a round costs `start`, and a step of K `alone` with one workgroup on a CU, `full` with `beside`.  A tile's steps wait
+// for weights from memory where few tiles share them.  Fitted to calls of 16 to 128 steps with weights out of the caches,
+// M of 1 to 8192; the choice is within 10% of the fastest of the kernels at all but a few of those sizes.
 struct Cost {
   int bn, bm, beside;
   float start, alone, full;
   float of(const LinearArgs& a) const {
-    const int64_t groups = (int64_t)((a.n + bn - 1) / bn) * ((a.m + bm - 1) / bm), each_cu = (groups + 255) / 256;
+    const int tiles_m = (a.m + bm - 1) / bm;
+    const int64_t groups = (int64_t)((a.n + bn - 1) / bn) * tiles_m, most = (groups + 255) / 256;  // most on a CU
     if (groups > (int64_t)1 << 22) return 1e30f;  // (launches of up to 2^32 - 1 threads)
-    const int64_t rounds = each_cu / beside, rest = each_cu % beside;
-    const float steps = (float)blocks_of(a.k), part = beside > 1 ? (full - alone) / (beside - 1) : 0.0f;
-    const float round = start + steps * full;
-    return rounds * round + (rest ? start + steps * (alone + part * (rest - 1)) : 0.0f) - (beside == 1 && rounds == 1 ? steps * (full - alone) : 0.0f);
+    const int64_t rounds = most / beside, rest = most % beside;
+    const float far = bn < 64 ? 1.0f : tiles_m == 1 ? 1.6f : tiles_m == 2 ? 1.25f : 1.0f;
+    const float steps = (float)blocks_of(a.k) * far, more = beside > 1 ? (full - alone) / (beside - 1) : 0.0f;
+    if (most == 1) return start + steps * alone;
+    return rounds * (start + steps * full) + (rest ? start + steps * (alone + more * (rest - 1)) : 0.0f);
   }
 };
 
@@ -387,22 +419,26 @@ hipError_t launch_typed(const LinearArgs& a, hipStream_t stream) {
 #ifdef PROBE_TILE
   if constexpr (sizeof(Out) == 2) return launch_tiles<Out, Codes, PROBE_TILE>(a, stream);
 #endif
-  constexpr Cost rows16x8{16, 8, 2, 2.8f, 0.062f, 0.13f}, rows32x16{32, 16, 1, 2.8f, 0.10f, 0.13f}, rows16x32{16, 32, 1, 3.0f, 0.075f, 0.075f},
-      rows32x32{32, 32, 1, 3.0f, 0.11f, 0.17f}, tiles64{64, 64, 2, 2.3f, 0.33f, 0.42f}, tiles128x64{128, 64, 3, 2.8f, 0.55f, 0.85f},
-      tiles128{128, 128, 2, 1.8f, 0.69f, 1.13f}, tiles256{256, 256, 1, 5.0f, 1.32f, 1.72f};
-  const Cost* const costs[] = {&rows16x8, &rows32x16, &rows16x32, &rows32x32, &tiles64, &tiles128x64, &tiles128, &tiles256};
-  constexpr int count = sizeof(Out) == 2 ? 8 : 7;  // (256 x 256 tiles of widened operands do not fit the registers)
+  constexpr Cost costs[] = {
+      {16, 8, 2, 2.8f, 0.062f, 0.13f}, {32, 16, 1, 2.8f, 0.10f, 0.13f}, {16, 32, 1, 3.0f, 0.075f, 0.075f}, {32, 32, 1, 3.0f, 0.11f, 0.17f},
+      {32, 64, 1, 5.0f, 0.19f, 0.19f},                                                               // rows
+      {64, 64, 2, 2.3f, 0.30f, 0.42f}, {128, 64, 2, 3.0f, 0.46f, 0.72f}, {64, 128, 2, 3.0f, 0.45f, 0.71f},
+      {128, 128, 1, 3.5f, 0.55f, 0.59f}, {128, 128, 2, 2.5f, 0.86f, 1.13f}, {256, 256, 1, 5.0f, 1.35f, 1.72f}};  // tiles
+  constexpr int count = sizeof(Out) == 2 ? 11 : 10;  // (256 x 256 tiles of widened operands do not fit the registers)
   int best = 0;
   for (int i = 1; i < count; ++i)
-    if (costs[i]->of(a) < costs[best]->of(a)) best = i;
+    if (costs[i].of(a) < costs[best].of(a)) best = i;
   switch (best) {
     case 0: return launch_rows<Out, Codes, 1, 1, 8, 8, 3>(a, stream);
     case 1: return launch_rows<Out, Codes, 2, 1, 16, 8, 3>(a, stream);
     case 2: return launch_rows<Out, Codes, 1, 2, 32, 8, 3>(a, stream);
     case 3: return launch_rows<Out, Codes, 2, 2, 32, 4, 3>(a, stream);
-    case 4: return launch_tiles<Out, Codes, 64, 64, 2, 2, 4>(a, stream);
-    case 5: return launch_tiles<Out, Codes, 128, 64, 2, 2, 2>(a, stream);
-    case 6: return launch_tiles<Out, Codes, 128, 128, 2, 2, 2>(a, stream);
+    case 4: return launch_rows<Out, Codes, 2, 4, 64, 4, 3>(a, stream);
+    case 5: return launch_tiles<Out, Codes, 64, 64, 2, 2, 4>(a, stream);
+    case 6: return launch_tiles<Out, Codes, 128, 64, 2, 2, 3>(a, stream);
+    case 7: return launch_tiles<Out, Codes, 64, 128, 2, 2, 3>(a, stream);
+    case 8: return launch_tiles<Out, Codes, 128, 128, 2, 4, 4>(a, stream);
+    case 9: return launch_tiles<Out, Codes, 128, 128, 2, 2, 2>(a, stream);
     default:
       if constexpr (sizeof(Out) == 2) return launch_tiles<Out, Codes, 256, 256, 2, 4, 2>(a, stream);
       return hipErrorInvalidValue;
