@@ -121,7 +121,7 @@ def run_quantize(device, x, gated=False):
 @pytest.mark.parametrize("width", WIDTHS)
 def test_quantize(hip_device, width, dtype):
     rng = np.random.default_rng(width)
-    for rows in (1, 6, 33):
+    for rows in (1, 33, 67):
         x = (np.exp(2 * rng.standard_normal((rows, 1))) * rng.standard_normal((rows, 2 * width))).astype(dtype)
         print(f"[case] quantize {rows} x {width} {dtype}", flush=True)
         plain.check_codes(*run_quantize(hip_device, x[:, :width].copy()), x[:, :width].astype(np.float64), 0.0)
@@ -160,6 +160,12 @@ def test_gated_far_gates(hip_device):
     codes, scales = run_quantize(hip_device, x, True)
     plain.check_codes(codes, scales, plain.gated(x), 2.0 ** -14)
     assert (codes[0, :4] & 127 == 0).all()
+    # alone in its block a closed gate's value is what there is: down to the smallest scale and past it
+    for g, v in ((-79.5, 3.0), (-80.5, 3.0), (-88.0, -7.0), (-95.0, 2000.0), (-120.0, 60000.0), (-104.0, 1.0), (-60000.0, 60000.0)):
+        x = np.array([[g, v]], np.float16)
+        plain.check_codes(*run_quantize(hip_device, x, True), plain.gated(x), 2.0 ** -14)
+    x = np.array([[-150.0, 3e38], [-200.0, -1e30], [-700.0, 3e38], [-3e38, 3e38]], np.float32)
+    plain.check_codes(*run_quantize(hip_device, x, True), plain.gated(x), 2.0 ** -12)
 
 
 # ------------------------------------------------------------------ linear
