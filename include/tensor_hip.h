@@ -376,7 +376,7 @@ int32_t tensor_paged_attention_workspace_v1(int64_t tokens, int64_t requests, in
  *    2 weight       fp32 [width]
  *    3 out          fp16 or fp32 [rows, width]      (may be x, of the same type)
  *    4 residual_out as residual                     (may be residual)
- *    5 eps          scalar fp32, positive
+ *    5 eps          scalar fp32, 2^-100 at least
  */
 int32_t tensor_rms_norm_v1(const TensorCallV1 *call, TensorErrorV1 *error);
 

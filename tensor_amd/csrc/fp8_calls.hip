@@ -37,8 +37,8 @@ int32_t norm_call(const TensorCallV1* call, TensorErrorV1* error, bool codes) {
   tensor_fp8::NormArgs args{};
   const uint32_t bits = (uint32_t)last.scalar;
   std::memcpy(&args.eps, &bits, 4);
-  if (!std::isfinite(args.eps) || args.eps <= 0.0f)
-    return fail(error, TENSOR_ERROR_ARGUMENT, "eps: must be positive and finite");
+  if (!std::isfinite(args.eps) || args.eps < tensor_fp8::kNormLeastEps)
+    return fail(error, TENSOR_ERROR_ARGUMENT, "eps: must be finite and 2^-100 at least");
   int64_t x[2] = {-1, -1};
   CHECK(check_values(a[0], "x", ordinal, x, 2, error));
   int64_t width[1] = {x[1]};

@@ -9,6 +9,7 @@ namespace tensor_fp8 {
 
 constexpr int kBlock = 128;           // values of a row that share a scale; rows of weights that do
 constexpr int kNormMaxWidth = 32768;  // a row is held in registers
+constexpr float kNormLeastEps = 0x1p-100f;  // squares that are lost below fp32 are lost beside it too
 // A launch has at most 2^32 - 1 threads along x.
 constexpr int64_t kMostThreads = ((int64_t)1 << 32) - 1;
 constexpr int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }

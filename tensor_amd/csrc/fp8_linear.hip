@@ -413,12 +413,6 @@ struct Cost {
 
 template <typename Out, typename Codes>
 hipError_t launch_typed(const LinearArgs& a, hipStream_t stream) {
-#ifdef PROBE_ROWS
-  return launch_rows<Out, Codes, PROBE_ROWS>(a, stream);
-#endif
-#ifdef PROBE_TILE
-  if constexpr (sizeof(Out) == 2) return launch_tiles<Out, Codes, PROBE_TILE>(a, stream);
-#endif
   constexpr Cost costs[] = {
       {16, 8, 2, 2.8f, 0.062f, 0.13f}, {32, 16, 1, 2.8f, 0.10f, 0.13f}, {16, 32, 1, 3.0f, 0.075f, 0.075f}, {32, 32, 1, 3.0f, 0.11f, 0.17f},
       {32, 64, 1, 5.0f, 0.19f, 0.19f},                                                               // rows

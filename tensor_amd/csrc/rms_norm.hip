@@ -64,8 +64,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(const NormArgs 
       if (chunk.has(e)) sum += h[c][e] * h[c][e];
   }
   sum = row_sum<T>(sum, part);
-  float eps = a.eps;
-  if (!(sum < kInfinity)) {  // squares past fp32: the same of h 2^-80, whose eps is lost beside it
+  float mean = sum / (float)a.width + a.eps;
+  if (!(mean < kInfinity)) {  // squares past fp32: the same of h 2^-80
     sum = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -76,9 +76,9 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(const NormArgs 
         if (chunk.has(e)) sum += h[c][e] * h[c][e];
     }
     sum = row_sum<T>(sum, part);
-    eps = 0.0f;
+    mean = sum / (float)a.width + a.eps * 0x1p-80f * 0x1p-80f;
   }
-  const float inverse = rsqrtf(sum / (float)a.width + eps);
+  const float inverse = rsqrtf(mean);
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int column = 8 * (t + T * c);

@@ -29,6 +29,7 @@ BLOCK = 128            # columns of a row that share a scale, and rows of weight
 LARGEST = 448.0        # of e4m3
 SMALLEST_SCALE = 2.0 ** -126
 NORM_MAX_WIDTH = 32768
+NORM_LEAST_EPS = 2.0 ** -100
 
 
 def _result(kernel: str, *arguments, **more) -> dict:
@@ -49,8 +50,8 @@ def _norm(kernel: str, dtype, residual, out_dtype, eps) -> dict:
     dtype = _dtype("dtype", dtype)
     if residual is not None:
         residual = _dtype("residual", residual)
-    if not (isinstance(eps, (int, float)) and not isinstance(eps, bool) and 0.0 < np.float32(eps) < np.inf):
-        raise ValueError("eps must be a positive finite number")
+    if not (isinstance(eps, (int, float)) and not isinstance(eps, bool) and NORM_LEAST_EPS <= np.float32(eps) < np.inf):
+        raise ValueError("eps must be a finite number, 2^-100 at least")
     arguments = [_buffer("x", dtype, "M", "D")]
     if residual is not None:
         arguments.append(_buffer("residual", residual, "M", "D"))

@@ -165,6 +165,16 @@ def test_refusals_of_values():
     assert call.run()[0] == ERR_ARG
 
 
+def test_least_eps():
+    assert builtin.manifest("rms_norm", eps=2.0 ** -100)
+    with pytest.raises(ValueError, match="eps"):
+        builtin.manifest("rms_norm", eps=2.0 ** -101)
+    call = norm()
+    call.args[call.index["eps"]].scalar = int(np.float32(2.0 ** -101).view(np.uint32))
+    status, message = call.run()
+    assert status == ERR_ARG and "eps" in message
+
+
 def test_refusals_of_sizes():
     call = norm()
     for name, shape in (("x", (1, 32769)), ("weight", (32769,)), ("out", (1, 32769))):

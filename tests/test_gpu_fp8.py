@@ -78,6 +78,16 @@ def test_norm_of_small_large_and_other_values(hip_device, width, out):
     assert np.isnan(plain.value(got[0])[4] if out == "codes" else got[0][4]).all()
 
 
+@pytest.mark.parametrize("width", [1, 5, 300, 9000])
+def test_norm_of_the_largest_and_least_eps(hip_device, width):
+    """Beside squares whose sum passes fp32, and beside such as are lost below it."""
+    rng = np.random.default_rng(width)
+    weight = np.ones(width, np.float32)
+    for size, eps in ((1e19, 1e38), (1e19, 1e36), (1.5e19, 3e38), (1e18, 3e38), (1e-15, 2.0 ** -100), (1e-25, 2.0 ** -100)):
+        x = (size * rng.uniform(0.8, 1.2, (3, width))).astype(np.float32)
+        check_norm(hip_device, x, None, weight, eps, "float32")
+
+
 def test_norm_sums_are_not_rounded_before_the_norm(hip_device):
     """Sums next to each other in fp16 differ in the result: h enters in fp32."""
     x = np.full((1, 128), 2048, np.float16)
