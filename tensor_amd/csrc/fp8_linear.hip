@@ -98,17 +98,19 @@ struct Units {
   }
 };
 
-// A tile of BN weight rows x BM activation rows by WN x WM waves, K in steps of a block through STAGES places of LDS.
-template <typename Out, typename Codes, int BN, int BM, int WN, int WM, int STAGES>
-__global__ __launch_bounds__(64 * WN * WM, 2) void linear_tiles(const LinearArgs a, int tiles_n, int tiles_m) {
+// A tile of BN weight rows x BM activation rows by WN x WM waves, K in steps of a block through STAGES places of LDS, which
+// LOADERS waves more fill (none: the waves themselves do).
+template <typename Out, typename Codes, int BN, int BM, int WN, int WM, int STAGES, int LOADERS>
+__global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(const LinearArgs a, int tiles_n, int tiles_m) {
   constexpr int NW = WN * WM, TN = BN / WN / 16, TM = BM / WM / 16;
-  constexpr int PW = BN / 8 / NW, PX = BM / 8 / NW;            // loads of a wave and step: 8 rows of 128 bytes each
-  constexpr int SCALES = BM < 64 ? 64 : BM;
-  constexpr int STAGE = (BN + BM) * 128 + 4 * SCALES;
-  static_assert(PW * 8 * NW == BN && PX * 8 * NW == BM, "whole loads for each wave");
+  constexpr int LW = LOADERS ? LOADERS : NW, PW = BN / 8 / LW, PX = BM / 8 / LW;  // loads of a wave and step: 8 rows of 128 bytes each
+  constexpr int PIECES = BM / 64 + 1;                                             // of scales: 64 of x each, those of w
+  constexpr int W = 128 * BN, X = 128 * BM, S = 256 * PIECES, STAGE = W + X + S;
+  static_assert(PW * 8 * LW == BN && PX * 8 * LW == BM && PIECES <= LW && BM % 64 == 0, "whole loads for each wave");
   static_assert(BN / WN <= 128, "a wave's weight rows share a scale");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * STAGE];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), quad = lane >> 4;
+  const int loader = LOADERS ? max(wave - NW, 0) : wave;
 
   // Workgroups go round the eight XCDs in turn: each XCD has a range of the tiles, eight of x by all of w at a time.
   const int total = tiles_n * tiles_m, share = (total + 7) / 8;
@@ -124,10 +126,10 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tiles(const LinearArgs
   // chunk, swizzled by the row, which is where LDS reads look for it.  Rows past the end are among the last eight.
   // (256 x 256 tiles keep the two apart: registers are what their waves have least of.  The others add them up once,
   // which spares scalar instructions at every load: 2048 x 4096 x 4096 in 34.9 us, 35.5.)
-  constexpr bool HELD = BN * BM < 256 * 256;
+  constexpr bool HELD = !LOADERS && BN * BM < 256 * 256;
   constexpr int PARTS = PW + PX + 1;
   const int chunk = (lane & 7) ^ (lane >> 3);
-  const int row_w = min(n0 + 8 * PW * wave, (a.n - 1) & ~7), row_x = min(m0 + 8 * PX * wave, (a.m - 1) & ~7);
+  const int row_w = min(n0 + 8 * PW * loader, (a.n - 1) & ~7), row_x = min(m0 + 8 * PX * loader, (a.m - 1) & ~7);
   const int left_w = a.n - row_w, left_x = a.m - row_x;
   const uint32_t lane_at = __umul24(lane >> 3, a.k) + 16 * chunk;
   const uint32_t edge_w = __umul24(min(lane >> 3, (a.n - 1) & 7), a.k) + 16 * chunk,
@@ -140,22 +142,25 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tiles(const LinearArgs
   };
   uint32_t held[HELD ? PARTS - 1 : 1];
   if constexpr (HELD) each<PARTS - 1>([&](auto p) { held[p] = first_of(p) + lane_of(p); });
-  const int part = 64 * (wave % (SCALES / 64));
-  const uint32_t s_at = 4 * min(part + lane, a.m - m0 - 1);
+  const int piece = loader % PIECES, block_n = n0 / kBlock;
+  const bool of_w = piece == PIECES - 1;
+  const uint32_t s_at = of_w ? 4 * steps * min(min(lane, (BN - 1) / kBlock), (a.n - 1) / kBlock - block_n)
+                             : 4 * min(64 * piece + lane, a.m - m0 - 1);
+  const int64_t s_next_at = of_w ? 1 : a.m;  // from one block of K to the next
   // weights of all stages, then activations, then scales: whatever the stage, reads are within an instruction's offset
-  constexpr int W = 128 * BN, X = 128 * BM, S = 4 * SCALES, X_AT = STAGES * W, S_AT = STAGES * (W + X);
-  const uint32_t lds_w = lds_address(lds) + 1024 * wave * PW, lds_x = lds_address(lds) + X_AT + 1024 * wave * PX,
-                 lds_s = lds_address(lds) + S_AT + 4 * part;
+  constexpr int X_AT = STAGES * W, S_AT = STAGES * (W + X);
+  const uint32_t lds_w = lds_address(lds) + 1024 * loader * PW, lds_x = lds_address(lds) + X_AT + 1024 * loader * PX,
+                 lds_s = lds_address(lds) + S_AT + 256 * piece;
   // The next stage to be loaded: its columns and its scales; `load` does part p of it, into place s (LAST: it may be
   // the last one, whose columns past the row's end are read from its last chunk and cleared below).
   const uint8_t *w = a.w + (size_t)row_w * a.k, *x = a.x + (size_t)row_x * a.k;
-  const float* x_scale = a.x_scales + m0;
+  const float* s_from = of_w ? a.w_scales + (size_t)block_n * steps : a.x_scales + m0;
   auto load = [&](int t, auto s, int p, auto last) {
     if (p == PW + PX) {
-      dma4(x_scale, s_at, lds_s + s * S);
+      dma4(s_from, s_at, lds_s + s * S);
       w += kBlock;
       x += kBlock;
-      x_scale += a.m;
+      s_from += s_next_at;
       return;
     }
     const uint32_t first = HELD ? 0 : first_of(p);
@@ -172,118 +177,138 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_tiles(const LinearArgs
     if (t * kBlock + 16 * chunk < a.k) return;
 #pragma unroll
     for (int j = 0; j < PW + PX; ++j) {
-      const int s = t % STAGES, at = j < PW ? s * W + 1024 * (wave * PW + j) : X_AT + s * X + 1024 * (wave * PX + j - PW);
+      const int s = t % STAGES, at = j < PW ? s * W + 1024 * (loader * PW + j) : X_AT + s * X + 1024 * (loader * PX + j - PW);
       *reinterpret_cast<uint4*>(lds + at + 16 * lane) = uint4{};
     }
   };
 
-  const int wn = wave % WN, wm = wave / WN;
-  // the present step's scale of the wave's weight rows
-  const Constant* w_scale = (const Constant*)(uintptr_t)a.w_scales + (size_t)min((n0 + wn * 16 * TN) / kBlock, (a.n - 1) / kBlock) * steps;
-  float4_t acc[TN][TM] = {};
-  // Products one after another, each followed by the scaled sum of the one DEEP - 1 before it, whose result is there by
-  // then.  The first half of the wave's weight groups goes by groups; by its end all of the second half is in registers,
-  // the next stage takes this one's place, and the second half goes by activation rows, each of which makes
-  // room for the next step's: LDS reads are spread over the step.
-  constexpr int DEEP = 3, HALF = TN / 2, APART = BN == 256 ? 7 : 0;
-  using Order = Units<TN, TM>;
-  constexpr int UNITS = Order::COUNT;
-  Codes xs[TM], ws[Order::SLOTS];
-  float scale[TM], next_scale[TM];
-  float4_t sums[DEEP];
-  // this lane's two chunks of a staged row, of the wave's first weight and activation rows; its first scale
-  const int at0 = 128 * (lane & 15) + 16 * (quad ^ (lane & 7)), at1 = 128 * (lane & 15) + 16 * ((4 + quad) ^ (lane & 7));
-  const uint8_t *const w0 = lds + 2048 * wn * TN + at0, *const w1 = lds + 2048 * wn * TN + at1;
-  const uint8_t *const x0 = lds + X_AT + 2048 * wm * TM + at0, *const x1 = lds + X_AT + 2048 * wm * TM + at1;
-  const uint8_t* const s0 = lds + S_AT + 4 * (16 * wm * TM + (lane & 15));
-  auto read_w = [&](auto s, int i) {
-    ws[Order::slot(i)].set(*reinterpret_cast<const uint4*>(w0 + s * W + 2048 * i), *reinterpret_cast<const uint4*>(w1 + s * W + 2048 * i));
-  };
-  auto read_x = [&](auto s, int j) {
-    xs[j].set(*reinterpret_cast<const uint4*>(x0 + s * X + 2048 * j), *reinterpret_cast<const uint4*>(x1 + s * X + 2048 * j));
-    next_scale[j] = *reinterpret_cast<const float*>(s0 + s * S + 64 * j);
-  };
-  // Waits until stage t has landed, this wave's part and after the barrier everyone's.
+  // Waits until this wave's part of stage t has landed, and with the barrier everyone's.
   auto landed = [&](int t, int issued) {
     if (STAGES > 2 && issued < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * PARTS) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (t + 1 == steps) clear_past(t);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
-  float sw = *w_scale;
+  if (!LOADERS || wave >= NW) {
+    each<STAGES - 1>([&](auto t) { if (t < steps) load_all(t, t); });
+    landed(0, STAGES - 2);
+    if (STAGES - 1 < steps) load_all(STAGES - 1, std::integral_constant<int, STAGES - 1>{});
+    if (LOADERS) {  // (a barrier for each of a step's)
+#pragma unroll 1
+      for (int t = 0; t < steps; ++t) {
+        landed(t + 1, t + STAGES - 1);
+        if (t + STAGES < steps) load_all(t + STAGES, t % STAGES);
+      }
+      return;
+    }
+  } else {
+    asm volatile("s_barrier" ::: "memory");
+  }
+
+  const int wn = wave % WN, wm = wave / WN;
+  float4_t acc[TN][TM] = {};
+  // Products one after another, each followed by the scaled sum of the one LAG before it, whose result is there by then:
+  // the last ones' in the next step (CARRY), or at the end of theirs, where registers are short.  The first half of the wave's weight groups goes by groups; by its end all of the second half is in registers,
+  // the next stage takes this one's place, and the second half goes by activation rows, each of which makes
+  // room for the next step's: LDS reads are spread over the step.
+  constexpr int LAG = 2, HALF = TN / 2, APART = BN == 256 ? 7 : 0;
+  constexpr bool CARRY = TN * TM <= 16;
+  constexpr int SUMS = CARRY ? 4 : LAG + 1;
+  using Order = Units<TN, TM>;
+  constexpr int UNITS = Order::COUNT;
+  Codes xs[TM], ws[Order::SLOTS];
+  float scale[TM] = {}, next_scale[TM], next_sw;
+  float4_t sums[SUMS] = {};
+  // this lane's two chunks of a staged row, of the wave's first weight and activation rows; its first scale
+  const int at0 = 128 * (lane & 15) + 16 * (quad ^ (lane & 7)), at1 = 128 * (lane & 15) + 16 * ((4 + quad) ^ (lane & 7));
+  const uint8_t *const w0 = lds + 2048 * wn * TN + at0, *const w1 = lds + 2048 * wn * TN + at1;
+  const uint8_t *const x0 = lds + X_AT + 2048 * wm * TM + at0, *const x1 = lds + X_AT + 2048 * wm * TM + at1;
+  const uint8_t* const s0 = lds + S_AT + 4 * (16 * wm * TM + (lane & 15));
+  const uint8_t* const sw0 = lds + S_AT + 256 * (PIECES - 1) + 4 * (wn * 16 * TN / kBlock);
+  auto read_w = [&](auto s, int i) {
+    ws[Order::slot(i)].set(*reinterpret_cast<const uint4*>(w0 + s * W + 2048 * i), *reinterpret_cast<const uint4*>(w1 + s * W + 2048 * i));
+  };
+  auto read_x = [&](auto s, int j) {
+    xs[j].set(*reinterpret_cast<const uint4*>(x0 + s * X + 2048 * j), *reinterpret_cast<const uint4*>(x1 + s * X + 2048 * j));
+    if (!CARRY) next_scale[j] = *reinterpret_cast<const float*>(s0 + s * S + 64 * j);
+  };
+  auto read_scales = [&](auto s) {
+    next_sw = *reinterpret_cast<const float*>(sw0 + s * S);
+    if constexpr (CARRY) each<TM>([&](auto j) { next_scale[j] = *reinterpret_cast<const float*>(s0 + s * S + 64 * j); });
+  };
+  auto take_scales = [&] { each<TM>([&](auto j) { scale[j] = next_scale[j] * next_sw; }); };
+  auto add = [&](auto v) {
+    constexpr int i = Order::group(v), j = Order::row(v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[i][j][e] += sums[v % SUMS][e] * scale[j];
+    asm volatile("" : "+v"(acc[i][j]));  // made here, not where it is used
+  };
   // Step t, whose stage is in place s.  LAST: the steps from which on less than STAGES follow.
-  auto step = [&](int t, auto s, auto s_next, int ahead, auto last) {
+  auto step = [&](int t, auto s, auto s_next, auto last) {
     constexpr bool LAST = decltype(last)::value;
-    float next_sw = w_scale[ahead];
-    each<TM>([&](auto j) { scale[j] = next_scale[j] * sw; });
-    each<UNITS + DEEP - 1>([&](auto unit) {
+    if constexpr (!CARRY) take_scales();
+    each<UNITS + (CARRY ? 0 : LAG)>([&](auto unit) {
       constexpr int u = decltype(unit)::value;
       if constexpr (u == HALF * TM) {  // (after the barrier nobody reads stage t any more)
-        if constexpr (LAST) landed(t + 1, t + STAGES - 1);
+        if constexpr (LOADERS) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else if constexpr (LAST) landed(t + 1, t + STAGES - 1);
         else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * PARTS) : "memory");
-        asm volatile("" : "+s"(next_sw));
+        read_scales(s_next);
         read_w(s_next, 0);
         if constexpr (TN == 4) read_w(s_next, 1);
       }
       if constexpr (u < UNITS) {
         constexpr int i = Order::group(u), j = Order::row(u);
-        if constexpr (u >= HALF * TM) {
+        if constexpr (!LOADERS && u >= HALF * TM) {
           if (!LAST || t + STAGES < steps)
             each<PARTS>([&](auto p) {
               if constexpr (least(decltype(p)::value * APART / 4, UNITS - HALF * TM - 1) == u - HALF * TM) load(t + STAGES, s, p, last);
             });
         }
-        sums[u % DEEP] = products(ws[Order::slot(i)], xs[j]);
+        sums[u % SUMS] = products(ws[Order::slot(i)], xs[j]);
         constexpr int r = Order::reads(u);
         if constexpr (r >= TN) read_w(s_next, r - TN);
         else if constexpr (r >= 0) read_w(s, r);
         if constexpr (i == TN - 1) read_x(s_next, j);
       }
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (u >= DEEP - 1) {
-        constexpr int v = u - DEEP + 1, i = Order::group(v), j = Order::row(v);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] += sums[v % DEEP][e] * scale[j];
-        asm volatile("" : "+v"(acc[i][j]));  // made here, not where it is used
-      }
+      if constexpr (u >= LAG) add(std::integral_constant<int, u - LAG>{});
+      else if constexpr (CARRY) add(std::integral_constant<int, UNITS + u - LAG>{});
+      if constexpr (CARRY && u == LAG - 1) take_scales();
       __builtin_amdgcn_sched_barrier(0);
     });
-    sw = next_sw;
   };
-  each<STAGES - 1>([&](auto t) { if (t < steps) load_all(t, t); });
-  landed(0, STAGES - 2);
-  if (STAGES - 1 < steps) load_all(STAGES - 1, std::integral_constant<int, STAGES - 1>{});
   constexpr std::integral_constant<int, 0> first_place{};
+  read_scales(first_place);
   each<Order::EARLY>([&](auto i) { read_w(first_place, i); });
   each<TM>([&](auto j) { read_x(first_place, j); });
   int t = 0;
-  for (; t + 2 * STAGES <= steps - 1; t += STAGES) {
+  for (; t + (LOADERS ? STAGES : 2 * STAGES + 1) <= steps; t += STAGES) {
     each<STAGES>([&](auto s) {
       constexpr int next = (decltype(s)::value + 1) % STAGES;
-      step(t + s, s, std::integral_constant<int, next>{}, s + 1, std::false_type{});
+      step(t + s, s, std::integral_constant<int, next>{}, std::false_type{});
     });
-    w_scale += STAGES;
   }
 #pragma unroll 1
-  for (; t < steps; ++t) {
-    step(t, t % STAGES, (t + 1) % STAGES, t + 1 < steps ? 1 : 0, std::true_type{});
-    ++w_scale;
-  }
+  for (; t < steps; ++t) step(t, t % STAGES, (t + 1) % STAGES, std::true_type{});
+  if constexpr (CARRY) each<LAG>([&](auto v) { add(std::integral_constant<int, UNITS - LAG + decltype(v)::value>{}); });
   // 16 activation rows at a time through LDS, a place for each wave, so that stores are of 16 bytes a lane and whole
   // lines.  (Past the last step's barrier nobody needs what a stage holds.)
   constexpr int COLUMNS = 16 * TN, PER = 16 / sizeof(Out), ROW = COLUMNS + PER;  // (rows shifted by four banks each)
   static_assert(NW * 16 * ROW * sizeof(Out) <= STAGES * STAGE, "a wave's place");
   typedef Out Out4 __attribute__((ext_vector_type(4)));
   typedef Out Chunk __attribute__((ext_vector_type(PER)));
+  int at_end = lane;
+  asm volatile("" : "+v"(at_end));  // what follows from it is worked out here, where registers are free
   Out* const own = reinterpret_cast<Out*>(lds) + wave * 16 * ROW;
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
 #pragma unroll
     for (int i = 0; i < TN; ++i)
-      *reinterpret_cast<Out4*>(own + (lane & 15) * ROW + 16 * i + 4 * quad) = __builtin_convertvector(acc[i][j], Out4);
+      *reinterpret_cast<Out4*>(own + (at_end & 15) * ROW + 16 * i + 4 * (at_end >> 4)) = __builtin_convertvector(acc[i][j], Out4);
 #pragma unroll
     for (int r = 0; r < 16 * COLUMNS / PER / 64; ++r) {
-      const int at = 64 * r + lane, row = at / (COLUMNS / PER), column = at % (COLUMNS / PER) * PER;
+      const int at = 64 * r + at_end, row = at / (COLUMNS / PER), column = at % (COLUMNS / PER) * PER;
       const Chunk v = *reinterpret_cast<const Chunk*>(own + row * ROW + column);
       const int m = m0 + wm * 16 * TM + 16 * j + row, n = n0 + wn * 16 * TN + column;
       if (m >= a.m || n >= a.n) continue;
@@ -393,65 +418,90 @@ hipError_t launch_rows(const LinearArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename Out, typename Codes, int BN, int BM, int WN, int WM, int STAGES>
+template <typename Out, typename Codes, int BN, int BM, int WN, int WM, int STAGES, int LOADERS>
 hipError_t launch_tiles(const LinearArgs& a, hipStream_t stream) {
   const int tiles_n = (a.n + BN - 1) / BN, tiles_m = (a.m + BM - 1) / BM;
   const int64_t total = (int64_t)tiles_n * tiles_m;
-  hipLaunchKernelGGL((linear_tiles<Out, Codes, BN, BM, WN, WM, STAGES>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WN * WM), 0, stream, a, tiles_n, tiles_m);
+  hipLaunchKernelGGL((linear_tiles<Out, Codes, BN, BM, WN, WM, STAGES, LOADERS>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * (WN * WM + LOADERS)), 0, stream, a, tiles_n, tiles_m);
   return hipGetLastError();
 }
 
 // What a call would take in one of the kernels, in microseconds: workgroups go round the CUs, `beside` at a time on one of
-// them; a round costs `start`, and a step of K `alone` with one workgroup on a CU, `full` with `beside`.  A tile's steps wait
-// for weights from memory where few tiles share them.  Fitted to calls of 16 to 128 steps with weights out of the caches,
-// M of 1 to 8192; the choice is within 10% of the fastest of the kernels at all but a few of those sizes.
+// them; a round costs `start`, and a step of K `alone` with one workgroup on a CU, `full` with `beside`.  Fitted to calls
+// of 20 to 96 steps and 1 to 4096 rows with weights out of the caches; over 85 (fp16 results) and 48 of them (fp32) the kernel
+// chosen takes 0.4% longer than the fastest of them in the mean, 10% and 17% at the worst.
 struct Cost {
   int bn, bm, beside;
   float start, alone, full;
   float of(const LinearArgs& a) const {
-    const int tiles_m = (a.m + bm - 1) / bm;
-    const int64_t groups = (int64_t)((a.n + bn - 1) / bn) * tiles_m, most = (groups + 255) / 256;  // most on a CU
+    const int64_t groups = (int64_t)((a.n + bn - 1) / bn) * ((a.m + bm - 1) / bm), most = (groups + 255) / 256;  // most on a CU
     if (groups > (int64_t)1 << 22) return 1e30f;  // (launches of up to 2^32 - 1 threads)
     const int64_t rounds = most / beside, rest = most % beside;
-    const float far = bn < 64 ? 1.0f : tiles_m == 1 ? 1.6f : tiles_m == 2 ? 1.25f : 1.0f;
-    const float steps = (float)blocks_of(a.k) * far, more = beside > 1 ? (full - alone) / (beside - 1) : 0.0f;
+    const float steps = (float)blocks_of(a.k), more = beside > 1 ? (full - alone) / (beside - 1) : 0.0f;
     if (most == 1) return start + steps * alone;
     return rounds * (start + steps * full) + (rest ? start + steps * (alone + more * (rest - 1)) : 0.0f);
   }
 };
 
-template <typename Out, typename Codes>
-hipError_t launch_typed(const LinearArgs& a, hipStream_t stream) {
-  constexpr Cost costs[] = {
-      {16, 8, 2, 2.8f, 0.062f, 0.13f}, {32, 16, 1, 2.8f, 0.10f, 0.13f}, {16, 32, 1, 3.0f, 0.075f, 0.075f}, {32, 32, 1, 3.0f, 0.11f, 0.17f},
-      {32, 64, 1, 5.0f, 0.19f, 0.19f},                                                               // rows
-      {64, 64, 2, 2.3f, 0.30f, 0.42f}, {128, 64, 2, 3.0f, 0.46f, 0.72f}, {64, 128, 2, 3.0f, 0.45f, 0.71f},
-      {128, 128, 1, 3.5f, 0.55f, 0.59f}, {128, 128, 2, 2.5f, 0.86f, 1.13f}, {256, 256, 1, 5.0f, 1.45f, 1.62f}};  // tiles
-  constexpr int count = sizeof(Out) == 2 ? 11 : 10;  // (256 x 256 tiles of widened operands do not fit the registers)
+template <size_t N>
+int cheapest(const LinearArgs& a, const Cost (&costs)[N]) {
   int best = 0;
-  for (int i = 1; i < count; ++i)
+  for (int i = 1; i < (int)N; ++i)
     if (costs[i].of(a) < costs[best].of(a)) best = i;
-  switch (best) {
+  return best;
+}
+
+template <typename Out, typename Codes>
+hipError_t launch_rows_of(int kernel, const LinearArgs& a, hipStream_t stream) {
+  switch (kernel) {
     case 0: return launch_rows<Out, Codes, 1, 1, 8, 8, 3>(a, stream);
     case 1: return launch_rows<Out, Codes, 2, 1, 16, 8, 3>(a, stream);
     case 2: return launch_rows<Out, Codes, 1, 2, 32, 8, 3>(a, stream);
     case 3: return launch_rows<Out, Codes, 2, 2, 32, 4, 3>(a, stream);
-    case 4: return launch_rows<Out, Codes, 2, 4, 64, 4, 3>(a, stream);
-    case 5: return launch_tiles<Out, Codes, 64, 64, 2, 2, 4>(a, stream);
-    case 6: return launch_tiles<Out, Codes, 128, 64, 2, 2, 3>(a, stream);
-    case 7: return launch_tiles<Out, Codes, 64, 128, 2, 2, 3>(a, stream);
-    case 8: return launch_tiles<Out, Codes, 128, 128, 2, 4, 4>(a, stream);
-    case 9: return launch_tiles<Out, Codes, 128, 128, 2, 2, 2>(a, stream);
-    default:
-      if constexpr (sizeof(Out) == 2) return launch_tiles<Out, Codes, 256, 256, 2, 4, 2>(a, stream);
-      return hipErrorInvalidValue;
+    default: return launch_rows<Out, Codes, 2, 4, 64, 4, 3>(a, stream);
+  }
+}
+
+hipError_t launch_fp16(const LinearArgs& a, hipStream_t stream) {
+  constexpr Cost costs[] = {
+      {16, 8, 2, 1.0f, 0.124f, 0.142f}, {32, 16, 1, 1.8f, 0.142f, 0.117f}, {16, 32, 1, 1.8f, 0.131f, 0.101f},
+      {32, 32, 1, 2.4f, 0.163f, 0.155f}, {32, 64, 1, 4.5f, 0.20f, 0.173f},                                     // rows
+      {64, 64, 2, 3.6f, 0.27f, 0.53f}, {128, 64, 2, 4.1f, 0.49f, 0.74f}, {128, 128, 1, 7.1f, 0.53f, 0.47f},
+      {256, 128, 1, 11.1f, 0.76f, 0.72f}, {256, 256, 1, 12.0f, 1.44f, 1.38f}};                                 // tiles
+  const int kernel = cheapest(a, costs);
+  switch (kernel) {
+    case 5: return launch_tiles<_Float16, Codes8, 64, 64, 1, 4, 4, 4>(a, stream);
+    case 6: return launch_tiles<_Float16, Codes8, 128, 64, 2, 2, 3, 4>(a, stream);
+    case 7: return launch_tiles<_Float16, Codes8, 128, 128, 1, 4, 4, 4>(a, stream);
+    case 8: return launch_tiles<_Float16, Codes8, 256, 128, 2, 2, 3, 4>(a, stream);
+    case 9: return launch_tiles<_Float16, Codes8, 256, 256, 2, 4, 2, 0>(a, stream);
+    default: return launch_rows_of<_Float16, Codes8>(kernel, a, stream);
+  }
+}
+
+// (Widening the operands is work of the waves that multiply: where two workgroups fill a CU, loaders only take their turns.)
+hipError_t launch_fp32(const LinearArgs& a, hipStream_t stream) {
+  constexpr Cost costs[] = {
+      {16, 8, 2, 1.5f, 0.12f, 0.14f}, {32, 16, 1, 1.9f, 0.14f, 0.13f}, {16, 32, 1, 1.9f, 0.13f, 0.10f},
+      {32, 32, 1, 2.7f, 0.17f, 0.15f}, {32, 64, 1, 4.9f, 0.22f, 0.20f},                                        // rows
+      {64, 64, 2, 4.8f, 0.34f, 0.80f}, {64, 64, 2, 5.2f, 0.35f, 0.67f}, {128, 64, 2, 6.6f, 0.62f, 1.28f},
+      {128, 64, 2, 5.7f, 0.69f, 1.09f}, {128, 128, 1, 4.6f, 0.99f, 1.00f}, {128, 128, 2, 10.0f, 1.02f, 1.71f}};  // tiles
+  const int kernel = cheapest(a, costs);
+  switch (kernel) {
+    case 5: return launch_tiles<float, Codes16, 64, 64, 2, 2, 4, 4>(a, stream);
+    case 6: return launch_tiles<float, Codes16, 64, 64, 2, 2, 4, 0>(a, stream);
+    case 7: return launch_tiles<float, Codes16, 128, 64, 2, 2, 3, 4>(a, stream);
+    case 8: return launch_tiles<float, Codes16, 128, 64, 2, 2, 3, 0>(a, stream);
+    case 9: return launch_tiles<float, Codes16, 128, 128, 2, 4, 4, 4>(a, stream);
+    case 10: return launch_tiles<float, Codes16, 128, 128, 2, 2, 2, 0>(a, stream);
+    default: return launch_rows_of<float, Codes16>(kernel, a, stream);
   }
 }
 
 }  // namespace
 
 hipError_t launch_linear(const LinearArgs& a, hipStream_t stream) {
-  return a.out_f32 ? launch_typed<float, Codes16>(a, stream) : launch_typed<_Float16, Codes8>(a, stream);
+  return a.out_f32 ? launch_fp32(a, stream) : launch_fp16(a, stream);
 }
 
 }  // namespace tensor_fp8

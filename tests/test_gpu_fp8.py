@@ -236,6 +236,30 @@ def test_linear_of_whole_numbers_is_exact(hip_device, shape):
         assert np.array_equal(got, want.astype(np.float32).astype(np.float16))
 
 
+# Few steps of many columns: each of the kernels for one of the types at least, with rows and columns past its tiles' ends.
+WIDE = [(13, 4099, 528), (27, 2051, 528), (27, 4099, 48), (61, 4099, 2064), (61, 4099, 528), (1, 24590, 144), (1, 24590, 528),
+        (1, 24590, 2064), (77, 16390, 48), (77, 16390, 2064), (77, 16390, 528), (77, 8197, 4112), (150, 16390, 528),
+        (205, 16390, 272), (205, 16390, 784), (602, 24590, 400), (1283, 6150, 48), (1283, 6150, 528)]
+
+
+@pytest.mark.parametrize("out_dtype", ["float16", "float32"])
+@pytest.mark.parametrize("shape", WIDE, ids=str)
+def test_linear_of_many_columns(hip_device, shape, out_dtype):
+    print(f"[case] linear {shape} {out_dtype}", flush=True)
+    m, n, k = shape
+    call = operands(sum(shape), *shape)
+    got = run_linear(hip_device, *call, out_dtype)
+    rows = np.unique(np.concatenate([np.arange(min(m, 5)), np.arange(max(m - 5, 0), m), np.random.default_rng(1).integers(0, m, 6)]))
+    call, got = (call[0][rows], np.ascontiguousarray(call[1][:, rows]), *call[2:]), got[rows]
+    plain.check_linear(got, *plain.linear(*call), k, plain.cut_off(*call) if out_dtype == "float16" else 0.0)
+
+
+@pytest.mark.parametrize("shape", WIDE, ids=str)
+def test_linear_of_whole_numbers_and_many_columns_is_exact(hip_device, shape):
+    print(f"[case] linear {shape}", flush=True)
+    test_linear_of_whole_numbers_is_exact(hip_device, shape)
+
+
 @pytest.mark.parametrize("shape", [(1, 200, 400), (9, 200, 400), (40, 200, 400), (150, 300, 400), (600, 520, 400)], ids=str)
 def test_linear_codes_that_are_not_numbers(hip_device, shape):
     """A NaN of x is in its row, one of w in its column, and nowhere else; so are scales that are not finite."""
