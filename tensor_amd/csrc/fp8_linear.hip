@@ -1,6 +1,18 @@
 // Linear layer on 8-bit operands with a scale for each block of 128 (fp8_common.h):
 //   out[m, n] = sum_b (sx[b, m] sw[n / 128, b]) sum_{k in block b} x[m, k] w[n, k]
 // The inner sum is the matrix cores', the outer one fp32 vector arithmetic on its results.
+//
+// fp16 results: 16 x 16 x 128 products of the codes themselves.  Within each 8 columns those cut a product off at 2^-13 of
+// the largest power of two there (measured), which an fp16 result does not show and an fp32 result would: there the
+// codes are widened to fp16, exactly, and multiplied at half the rate.
+//
+// A step of K is one block, so each 16 x 16 sum of a step is scaled and added once: four vector instructions beside the 32
+// cycles of a product, on a SIMD where they overlap with other products.  What bounds a call:
+//   few rows (linear_rows): the weights' bytes.  1 x 24576 x 4096 in 19.7 us (5.1 TB/s), 16 x 4096 x 12288 in 10.2 (4.9).
+//   some hundred rows (linear_tiles, 64 x 64 to 256 x 128): a CU's LDS, and how many misses it has under way where weights come
+//     from memory.  333 x 6144 x 4096 in 14.5 us (1.15 PFLOP/s) with the weights in the last cache, 20.6 without.
+//   thousands (256 x 256): the matrix cores at the clock that their power allows, 1.9-2.0 GHz.  8192 x 24576 x 4096 in 690 us
+//     (2.39 PFLOP/s; on codes that are all zero a fifth faster).  fp32 results in 1370 us (1.2 PFLOP/s).
 #include <type_traits>
 #include <utility>
 
@@ -100,6 +112,15 @@ struct Units {
 
 // A tile of BN weight rows x BM activation rows by WN x WM waves, K in steps of a block through STAGES places of LDS, which
 // LOADERS waves more fill (none: the waves themselves do).
+//
+// A wave that loads waits while the CU takes its loads, and so do its products.  Four waves that do nothing else leave the
+// others to multiply, one on each SIMD, with larger tiles of their own, which read less of LDS, whose 128 bytes a
+// cycle are what a step takes (128 x 128 by eight waves of 64 x 32 that load as well: 98 KB read and 33 written, 0.42 us; by
+// four of 128 x 32: 82 and 33, 0.35 us).  333 x 6144 x 4096 in 14.5 us, 18.4 without such waves; 2048 x 4096 x 4096 in 31.7 by 256 x 128
+// tiles with them, 34.1 by 128 x 128 without.  Two waves of 256 x 256 tiles take a SIMD's registers: no room for a third.
+// Scales come through LDS as well: the wait of a scalar load would wait for every LDS read before it.
+// Prefetches into L2 ahead of the stages, K begun at another block by each workgroup, 32 x 32 x 64 products and more stages were
+// measured level or slower.
 template <typename Out, typename Codes, int BN, int BM, int WN, int WM, int STAGES, int LOADERS>
 __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(const LinearArgs a, int tiles_n, int tiles_m) {
   constexpr int NW = WN * WM, TN = BN / WN / 16, TM = BM / WM / 16;
@@ -124,9 +145,6 @@ __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(cons
   const int steps = (a.k + kBlock - 1) / kBlock;
   // A load is of 8 rows: where the first of them begins is the wave's, where in them a lane reads its own, its row and its
   // chunk, swizzled by the row, which is where LDS reads look for it.  Rows past the end are among the last eight.
-  // (256 x 256 tiles keep the two apart: registers are what their waves have least of.  The others add them up once,
-  // which spares scalar instructions at every load: 2048 x 4096 x 4096 in 34.9 us, 35.5.)
-  constexpr bool HELD = !LOADERS && BN * BM < 256 * 256;
   constexpr int PARTS = PW + PX + 1;
   const int chunk = (lane & 7) ^ (lane >> 3);
   const int row_w = min(n0 + 8 * PW * loader, (a.n - 1) & ~7), row_x = min(m0 + 8 * PX * loader, (a.m - 1) & ~7);
@@ -140,8 +158,6 @@ __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(cons
   auto lane_of = [&](int p) {
     return p < PW ? 8 * p + 8 <= left_w ? lane_at : edge_w : 8 * (p - PW) + 8 <= left_x ? lane_at : edge_x;
   };
-  uint32_t held[HELD ? PARTS - 1 : 1];
-  if constexpr (HELD) each<PARTS - 1>([&](auto p) { held[p] = first_of(p) + lane_of(p); });
   const int piece = loader % PIECES, block_n = n0 / kBlock;
   const bool of_w = piece == PIECES - 1;
   const uint32_t s_at = of_w ? 4 * steps * min(min(lane, (BN - 1) / kBlock), (a.n - 1) / kBlock - block_n)
@@ -163,11 +179,10 @@ __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(cons
       s_from += s_next_at;
       return;
     }
-    const uint32_t first = HELD ? 0 : first_of(p);
-    uint32_t at = HELD ? held[HELD ? p : 0] : lane_of(p);
+    uint32_t at = lane_of(p);
     if (decltype(last)::value) at -= max(16 * chunk - (a.k - t * kBlock - 16), 0);
-    if (p < PW) dma16(w + first, at, lds_w + s * W + 1024 * p);
-    else dma16(x + first, at, lds_x + s * X + 1024 * (p - PW));
+    if (p < PW) dma16(w + first_of(p), at, lds_w + s * W + 1024 * p);
+    else dma16(x + first_of(p), at, lds_x + s * X + 1024 * (p - PW));
   };
   auto load_all = [&](int t, auto s) {
     each<PARTS>([&](auto p) { load(t, s, p, std::true_type{}); });
@@ -324,7 +339,7 @@ __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(cons
   }
 }
 
-// Few activation rows (decode): 16 GN weight rows x 16 GM activation rows (of which XR are staged) by WAVES waves, each of
+// Few activation rows (decode), bound by the weights' bytes: 16 GN weight rows x 16 GM activation rows (of which XR are staged) by WAVES waves, each of
 // which streams its own steps of K through STAGES places of its own in LDS, without barriers; their sums meet at the end.
 template <typename Out, typename Codes, int GN, int GM, int XR, int WAVES, int STAGES>
 __global__ __launch_bounds__(64 * WAVES) void linear_rows(const LinearArgs a, int tiles_m) {

