@@ -227,31 +227,34 @@ __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(cons
   // the next stage takes this one's place, and the second half goes by activation rows, each of which makes
   // room for the next step's: LDS reads are spread over the step.
   constexpr int LAG = 2, HALF = TN / 2, APART = BN == 256 ? 7 : 0;
-  constexpr bool CARRY = TN * TM <= 16;
+  constexpr bool CARRY = TN * TM * sizeof(Codes) <= 512;
   constexpr int SUMS = CARRY ? 4 : LAG + 1;
   using Order = Units<TN, TM>;
   constexpr int UNITS = Order::COUNT;
   Codes xs[TM], ws[Order::SLOTS];
-  float scale[TM] = {}, next_scale[TM], next_sw;
+  float scale[TM] = {}, next_scale[TM], next_sw;  // of activation rows, times that of the wave's weights
   float4_t sums[SUMS] = {};
   // this lane's two chunks of a staged row, of the wave's first weight and activation rows; its first scale
   const int at0 = 128 * (lane & 15) + 16 * (quad ^ (lane & 7)), at1 = 128 * (lane & 15) + 16 * ((4 + quad) ^ (lane & 7));
   const uint8_t *const w0 = lds + 2048 * wn * TN + at0, *const w1 = lds + 2048 * wn * TN + at1;
   const uint8_t *const x0 = lds + X_AT + 2048 * wm * TM + at0, *const x1 = lds + X_AT + 2048 * wm * TM + at1;
-  const uint8_t* const s0 = lds + S_AT + 4 * (16 * wm * TM + (lane & 15));
-  const uint8_t* const sw0 = lds + S_AT + 256 * (PIECES - 1) + 4 * (wn * 16 * TN / kBlock);
+  // (Past an instruction's offset from the start of LDS, so registers of their own hold them, said so that they stay the only ones.)
+  uint32_t s0 = lds_address(lds) + S_AT + 4 * (16 * wm * TM + (lane & 15));
+  uint32_t sw0 = lds_address(lds) + S_AT + 256 * (PIECES - 1) + 4 * (wn * 16 * TN / kBlock);
+  asm volatile("" : "+v"(s0), "+v"(sw0));
+  auto scale_at = [&](uint32_t at) { return *(const float __attribute__((address_space(3)))*)at; };
   auto read_w = [&](auto s, int i) {
     ws[Order::slot(i)].set(*reinterpret_cast<const uint4*>(w0 + s * W + 2048 * i), *reinterpret_cast<const uint4*>(w1 + s * W + 2048 * i));
   };
   auto read_x = [&](auto s, int j) {
     xs[j].set(*reinterpret_cast<const uint4*>(x0 + s * X + 2048 * j), *reinterpret_cast<const uint4*>(x1 + s * X + 2048 * j));
-    if (!CARRY) next_scale[j] = *reinterpret_cast<const float*>(s0 + s * S + 64 * j);
   };
   auto read_scales = [&](auto s) {
-    next_sw = *reinterpret_cast<const float*>(sw0 + s * S);
-    if constexpr (CARRY) each<TM>([&](auto j) { next_scale[j] = *reinterpret_cast<const float*>(s0 + s * S + 64 * j); });
+    next_sw = scale_at(sw0 + s * S);
+    if constexpr (CARRY) each<TM>([&](auto j) { next_scale[j] = scale_at(s0 + s * S + 64 * j); });
   };
-  auto take_scales = [&] { each<TM>([&](auto j) { scale[j] = next_scale[j] * next_sw; }); };
+  auto read_scale = [&](auto s, int j) { scale[j] = scale_at(s0 + s * S + 64 * j); };  // (without CARRY)
+  auto take_scales = [&] { each<TM>([&](auto j) { scale[j] = (CARRY ? next_scale[j] : scale[j]) * next_sw; }); };
   auto add = [&](auto v) {
     constexpr int i = Order::group(v), j = Order::row(v);
 #pragma unroll
@@ -290,11 +293,14 @@ __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(cons
       if constexpr (u >= LAG) add(std::integral_constant<int, u - LAG>{});
       else if constexpr (CARRY) add(std::integral_constant<int, UNITS + u - LAG>{});
       if constexpr (CARRY && u == LAG - 1) take_scales();
+      if constexpr (!CARRY && u >= LAG)
+        if constexpr (Order::group(u - LAG) == TN - 1) read_scale(s_next, Order::row(u - LAG));
       __builtin_amdgcn_sched_barrier(0);
     });
   };
   constexpr std::integral_constant<int, 0> first_place{};
   read_scales(first_place);
+  if constexpr (!CARRY) each<TM>([&](auto j) { read_scale(first_place, j); });
   each<Order::EARLY>([&](auto i) { read_w(first_place, i); });
   each<TM>([&](auto j) { read_x(first_place, j); });
   int t = 0;
@@ -304,8 +310,14 @@ __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(cons
       step(t + s, s, std::integral_constant<int, next>{}, std::false_type{});
     });
   }
+  if constexpr (LOADERS) {
+    each<STAGES - 1>([&](auto s) {
+      if (t + s < steps) step(t + s, s, std::integral_constant<int, decltype(s)::value + 1>{}, std::true_type{});
+    });
+  } else {
 #pragma unroll 1
-  for (; t < steps; ++t) step(t, t % STAGES, (t + 1) % STAGES, std::true_type{});
+    for (; t < steps; ++t) step(t, t % STAGES, (t + 1) % STAGES, std::true_type{});
+  }
   if constexpr (CARRY) each<LAG>([&](auto v) { add(std::integral_constant<int, UNITS - LAG + decltype(v)::value>{}); });
   // 16 activation rows at a time through LDS, a place for each wave, so that stores are of 16 bytes a lane and whole
   // lines.  (Past the last step's barrier nobody needs what a stage holds.)
@@ -313,8 +325,9 @@ __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(cons
   static_assert(NW * 16 * ROW * sizeof(Out) <= STAGES * STAGE, "a wave's place");
   typedef Out Out4 __attribute__((ext_vector_type(4)));
   typedef Out Chunk __attribute__((ext_vector_type(PER)));
-  int at_end = lane;
-  asm volatile("" : "+v"(at_end));  // what follows from it is worked out here, where registers are free
+  uint32_t all = ~0u;
+  asm volatile("" : "+s"(all));  // the lane's number, and what follows from it, worked out here, where registers are free
+  const int at_end = __builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0));
   Out* const own = reinterpret_cast<Out*>(lds) + wave * 16 * ROW;
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
@@ -500,14 +513,14 @@ hipError_t launch_fp32(const LinearArgs& a, hipStream_t stream) {
       {16, 8, 2, 1.5f, 0.12f, 0.14f}, {32, 16, 1, 1.9f, 0.14f, 0.13f}, {16, 32, 1, 1.9f, 0.13f, 0.10f},
       {32, 32, 1, 2.7f, 0.17f, 0.15f}, {32, 64, 1, 4.9f, 0.22f, 0.20f},                                        // rows
       {64, 64, 2, 4.8f, 0.34f, 0.80f}, {64, 64, 2, 5.2f, 0.35f, 0.67f}, {128, 64, 2, 6.6f, 0.62f, 1.28f},
-      {128, 64, 2, 5.7f, 0.69f, 1.09f}, {128, 128, 1, 4.6f, 0.99f, 1.00f}, {128, 128, 2, 10.0f, 1.02f, 1.71f}};  // tiles
+      {128, 64, 2, 5.7f, 0.69f, 1.09f}, {128, 128, 1, 5.5f, 1.04f, 1.03f}, {128, 128, 2, 10.0f, 1.02f, 1.71f}};  // tiles
   const int kernel = cheapest(a, costs);
   switch (kernel) {
     case 5: return launch_tiles<float, Codes16, 64, 64, 2, 2, 4, 4>(a, stream);
     case 6: return launch_tiles<float, Codes16, 64, 64, 2, 2, 4, 0>(a, stream);
     case 7: return launch_tiles<float, Codes16, 128, 64, 2, 2, 3, 4>(a, stream);
     case 8: return launch_tiles<float, Codes16, 128, 64, 2, 2, 3, 0>(a, stream);
-    case 9: return launch_tiles<float, Codes16, 128, 128, 2, 4, 4, 4>(a, stream);
+    case 9: return launch_tiles<float, Codes16, 128, 128, 2, 2, 4, 4>(a, stream);
     case 10: return launch_tiles<float, Codes16, 128, 128, 2, 2, 2, 0>(a, stream);
     default: return launch_rows_of<float, Codes16>(kernel, a, stream);
   }
