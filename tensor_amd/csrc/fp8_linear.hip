@@ -9,10 +9,11 @@
 // A step of K is one block, so each 16 x 16 sum of a step is scaled and added once: four vector instructions beside the 32
 // cycles of a product, on a SIMD where they overlap with other products.  What bounds a call:
 //   few rows (linear_rows): the weights' bytes.  1 x 24576 x 4096 in 19.7 us (5.1 TB/s), 16 x 4096 x 12288 in 10.2 (4.9).
-//   some hundred rows (linear_tiles, 64 x 64 to 256 x 128): a CU's LDS, and how many misses it has under way where weights come
-//     from memory.  333 x 6144 x 4096 in 14.5 us (1.15 PFLOP/s) with the weights in the last cache, 20.6 without.
-//   thousands (256 x 256): the matrix cores at the clock that their power allows, 1.9-2.0 GHz.  8192 x 24576 x 4096 in 690 us
-//     (2.39 PFLOP/s; on codes that are all zero a fifth faster).  fp32 results in 1370 us (1.2 PFLOP/s).
+//   some hundred rows (linear_tiles, 64 x 64 to 256 x 128): a step's chain of LDS reads, products and barrier on the CUs
+//     that have a tile (0.35 us for 128 x 128, of which the products are 0.21), and where weights come from memory a
+//     CU's misses under way.  333 x 6144 x 4096 in 14.7 us (1.14 PFLOP/s) with the weights in the last cache, 20.9 without.
+//   thousands (256 x 256): the matrix cores, busy 60% of the cycles, at the clock that their power allows.
+//     8192 x 24576 x 4096 in 680 us (2.42 PFLOP/s; an eighth faster on codes that are all zero).  fp32 results in 1390 us.
 #include <type_traits>
 #include <utility>
 
@@ -95,7 +96,7 @@ __device__ __forceinline__ void each(F&& f) {
 template <int TN, int TM>
 struct Units {
   static constexpr int COUNT = TN * TM, HALF = TN / 2;
-  static_assert(TN == 8 || TN == 4 || TN == 2, "the places of weight groups");
+  static_assert((TN == 8 && TM > 1) || TN == 4 || TN == 2, "the places of weight groups");
   static constexpr int SLOTS = TN == 8 ? 5 : TN;
   static constexpr int EARLY = TN == 2 ? 1 : 2;  // groups read before the step
   static constexpr int group(int u) { return u < HALF * TM ? u / TM : HALF + (u - HALF * TM) % HALF; }
@@ -113,18 +114,18 @@ struct Units {
 // A tile of BN weight rows x BM activation rows by WN x WM waves, K in steps of a block through STAGES places of LDS, which
 // LOADERS waves more fill (none: the waves themselves do).
 //
-// A wave that loads waits while the CU takes its loads, and so do its products.  Four waves that do nothing else leave the
-// others to multiply, one on each SIMD, with larger tiles of their own, which read less of LDS, whose 128 bytes a
-// cycle are what a step takes (128 x 128 by eight waves of 64 x 32 that load as well: 98 KB read and 33 written, 0.42 us; by
-// four of 128 x 32: 82 and 33, 0.35 us).  333 x 6144 x 4096 in 14.5 us, 18.4 without such waves; 2048 x 4096 x 4096 in 31.7 by 256 x 128
-// tiles with them, 34.1 by 128 x 128 without.  Two waves of 256 x 256 tiles take a SIMD's registers: no room for a third.
+// A wave that loads waits while the CU takes its loads, and so do its products: eight waves of a 128 x 128 tile take 0.42 us a
+// step with loads and 0.33 without.  Four waves that do nothing else leave the others to multiply (0.33 again), one on each
+// SIMD, with larger tiles of their own.  333 x 6144 x 4096 takes 14.7 us, 18.4 without such waves; 2048 x 4096 x 4096
+// takes 30.9 by 256 x 128 tiles with them, 34.1 by 128 x 128 without.  Two waves of 256 x 256 tiles take a SIMD's
+// registers: no room for a third.
 // Scales come through LDS as well: the wait of a scalar load would wait for every LDS read before it.
 // Prefetches into L2 ahead of the stages, K begun at another block by each workgroup, 32 x 32 x 64 products and more stages were
 // measured level or slower.
 template <typename Out, typename Codes, int BN, int BM, int WN, int WM, int STAGES, int LOADERS>
 __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(const LinearArgs a, int tiles_n, int tiles_m) {
   constexpr int NW = WN * WM, TN = BN / WN / 16, TM = BM / WM / 16;
-  constexpr int LW = LOADERS ? LOADERS : NW, PW = BN / 8 / LW, PX = BM / 8 / LW;  // loads of a wave and step: 8 rows of 128 bytes each
+  constexpr int LW = LOADERS ? LOADERS : NW, PW = BN / 8 / LW, PX = BM / 8 / LW;  // a wave's loads in a step, of 8 rows each
   constexpr int PIECES = BM / 64 + 1;                                             // of scales: 64 of x each, those of w
   constexpr int W = 128 * BN, X = 128 * BM, S = 256 * PIECES, STAGE = W + X + S;
   static_assert(PW * 8 * LW == BN && PX * 8 * LW == BM && PIECES <= LW && BM % 64 == 0, "whole loads for each wave");
@@ -223,9 +224,9 @@ __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(cons
   const int wn = wave % WN, wm = wave / WN;
   float4_t acc[TN][TM] = {};
   // Products one after another, each followed by the scaled sum of the one LAG before it, whose result is there by then:
-  // the last ones' in the next step (CARRY), or at the end of theirs, where registers are short.  The first half of the wave's weight groups goes by groups; by its end all of the second half is in registers,
-  // the next stage takes this one's place, and the second half goes by activation rows, each of which makes
-  // room for the next step's: LDS reads are spread over the step.
+  // the last ones' in the next step (CARRY), or at the end of theirs, where registers are short.  The first half of the wave's
+  // weight groups goes by groups; by its end all of the second half is in registers, the next stage takes this one's place, and
+  // the second half goes by activation rows, each of which makes room for the next step's: LDS reads are spread over the step.
   constexpr int LAG = 2, HALF = TN / 2, APART = BN == 256 ? 7 : 0;
   constexpr bool CARRY = TN * TM * sizeof(Codes) <= 512;
   constexpr int SUMS = CARRY ? 4 : LAG + 1;
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(cons
   const int at0 = 128 * (lane & 15) + 16 * (quad ^ (lane & 7)), at1 = 128 * (lane & 15) + 16 * ((4 + quad) ^ (lane & 7));
   const uint8_t *const w0 = lds + 2048 * wn * TN + at0, *const w1 = lds + 2048 * wn * TN + at1;
   const uint8_t *const x0 = lds + X_AT + 2048 * wm * TM + at0, *const x1 = lds + X_AT + 2048 * wm * TM + at1;
-  // (Past an instruction's offset from the start of LDS, so registers of their own hold them, said so that they stay the only ones.)
+  // (Past an instruction's offset from the start of LDS: in a register each, and no second one beside it.)
   uint32_t s0 = lds_address(lds) + S_AT + 4 * (16 * wm * TM + (lane & 15));
   uint32_t sw0 = lds_address(lds) + S_AT + 256 * (PIECES - 1) + 4 * (wn * 16 * TN / kBlock);
   asm volatile("" : "+v"(s0), "+v"(sw0));
