@@ -157,6 +157,69 @@ def check_graph():
             assert torch.equal(last.outputs[0], want), (tokens, replay)
 
 
+def whole(n, k):
+    """Codes of 0, 1, 2 and their negatives: sums of up to 2^20 products are whole numbers below 2^22, exact in any order."""
+    codes = torch.tensor([0x00, 0x38, 0x40, 0xB8, 0xC0], dtype=torch.uint8, device="cuda")
+    return codes[torch.randint(0, 5, (n, k), device="cuda")]
+
+
+def ones(*shape):
+    return torch.ones(shape, device="cuda")
+
+
+def check_far():
+    """Places past 2^32 and the longest extents."""
+    for m, n, k, dtype in ((140001, 32770, 16, "float16"), (70001, 32770, 48, "float32"), (1 << 20, 40, 16, "float16"),
+                           (1, 1 << 22, 16, "float32"), (70, 1 << 22, 32, "float16")):
+        step(f"linear {m} x {n} x {k} {dtype}")
+        linear, x, w = tt.load("fp8_linear", out_dtype=dtype), whole(m, k), whole(n, k)
+        ws = ones(-(-n // 128), 1)
+        out = linear(x, ones(1, m), w, ws)
+        rows = torch.unique(torch.cat([torch.arange(min(m, 9)), torch.arange(max(m - 9, 0), m), torch.randint(0, m, (20,))])).cuda()
+        want = linear(x[rows], ones(1, len(rows)), w, ws)
+        assert torch.equal(out[rows], want)
+        columns = torch.unique(torch.cat([torch.arange(min(n, 9)), torch.arange(n - 9, n), torch.randint(0, n, (20,))])).cuda()
+        values = torch.from_numpy(plain.value(np.arange(256))).cuda()
+        exact = values[x[rows].long()] @ values[w[columns].long()].T
+        assert torch.equal(out[rows][:, columns].double(), exact)
+        del out, want
+    for dtype in ("float16", "float32"):
+        step(f"linear 3 x 130 x {1 << 20} {dtype}")
+        k = 1 << 20
+        x, w = whole(3, k), whole(130, k)
+        out = tt.load("fp8_linear", out_dtype=dtype)(x, ones(k // 128, 3), w, ones(2, k // 128))
+        values = torch.from_numpy(plain.value(np.arange(256))).cuda()
+        exact = values[x.long()] @ values[w.long()].T
+        assert torch.equal(out, exact.to(out.dtype))
+    step("gates of 110001 x 24576")
+    x = torch.randn((110001, 2 * 24576), device="cuda", dtype=torch.float16)
+    codes, scales = tt.load("quantize_fp8", gated=True)(x)
+    want, want_scales = tt.load("quantize_fp8", gated=True)(x[-100:])
+    assert torch.equal(codes[-100:], want) and torch.equal(scales[:, -100:], want_scales)
+    del codes, scales, want
+    step("norm of 220002 x 24576")
+    x = x.view(220002, 24576)
+    weight = torch.rand(24576, device="cuda")
+    out = tt.load("rms_norm")(x, weight)
+    assert torch.equal(out[-100:], tt.load("rms_norm")(x[-100:], weight))
+    del x, out
+    torch.cuda.empty_cache()
+
+
+def check_surroundings_of_tiles():
+    step("memory around the outputs of each kind of tile")
+    for m, n, k in ((1, 24590, 528), (1, 24590, 2064), (77, 16390, 528), (77, 8197, 4112), (150, 16390, 528), (205, 16390, 784),
+                    (1283, 6150, 528)):
+        x, w, xs, ws = whole(m, k), whole(n, k), ones(-(-k // 128), m), ones(-(-n // 128), -(-k // 128))
+        for dtype in ("float16", "float32"):
+            room = torch.full((m * n + 131072,), 7.0, dtype=getattr(torch, dtype), device="cuda")
+            out = room[65536:65536 + m * n].view(m, n)
+            linear = tt.load("fp8_linear", out_dtype=dtype)
+            linear.prepare(x, xs, w, ws, outputs=[out])()
+            assert torch.equal(out, linear(x, xs, w, ws))
+            assert bool((room[:65536] == 7.0).all()) and bool((room[65536 + m * n:] == 7.0).all()), (m, n, k)
+
+
 def check_example():
     # the weights are the codes' own; activations are rounded to 8 bits four times on the way (2^-4 at most, evenly spread
     # errors of 2^-4 / sqrt(3) in the 2-norm and less), and what they add to stays
@@ -171,6 +234,8 @@ if __name__ == "__main__":
     check_surroundings()
     check_streams()
     check_graph()
+    check_far()
+    check_surroundings_of_tiles()
     check_example()
     tt.close()
     print("[torch-fp8] ok", flush=True)
