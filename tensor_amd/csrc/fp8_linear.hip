@@ -79,8 +79,6 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t offset, uint32_t
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory");
 }
 
-constexpr int least(int a, int b) { return a < b ? a : b; }
-
 // f(0), f(1), .. f(N - 1), each with its number as a constant
 template <typename F, int... I>
 __device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
@@ -227,7 +225,7 @@ __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(cons
   // the last ones' in the next step (CARRY), or at the end of theirs, where registers are short.  The first half of the wave's
   // weight groups goes by groups; by its end all of the second half is in registers, the next stage takes this one's place, and
   // the second half goes by activation rows, each of which makes room for the next step's: LDS reads are spread over the step.
-  constexpr int LAG = 2, HALF = TN / 2, APART = BN == 256 ? 7 : 0;
+  constexpr int LAG = 2, HALF = TN / 2;
   constexpr bool CARRY = TN * TM * sizeof(Codes) <= 512;
   constexpr int SUMS = CARRY ? 4 : LAG + 1;
   using Order = Units<TN, TM>;
@@ -278,11 +276,8 @@ __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(cons
       }
       if constexpr (u < UNITS) {
         constexpr int i = Order::group(u), j = Order::row(u);
-        if constexpr (!LOADERS && u >= HALF * TM) {
-          if (!LAST || t + STAGES < steps)
-            each<PARTS>([&](auto p) {
-              if constexpr (least(decltype(p)::value * APART / 4, UNITS - HALF * TM - 1) == u - HALF * TM) load(t + STAGES, s, p, last);
-            });
+        if constexpr (!LOADERS && u == HALF * TM) {
+          if (!LAST || t + STAGES < steps) each<PARTS>([&](auto p) { load(t + STAGES, s, p, last); });
         }
         sums[u % SUMS] = products(ws[Order::slot(i)], xs[j]);
         constexpr int r = Order::reads(u);
