@@ -79,6 +79,8 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t offset, uint32_t
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory");
 }
 
+constexpr int least(int a, int b) { return a < b ? a : b; }
+
 // f(0), f(1), .. f(N - 1), each with its number as a constant
 template <typename F, int... I>
 __device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
@@ -276,8 +278,12 @@ __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(cons
       }
       if constexpr (u < UNITS) {
         constexpr int i = Order::group(u), j = Order::row(u);
-        if constexpr (!LOADERS && u == HALF * TM) {
-          if (!LAST || t + STAGES < steps) each<PARTS>([&](auto p) { load(t + STAGES, s, p, last); });
+        // one load beside two products (8192 x 24576 x 4096: 676 us, all at once 715)
+        if constexpr (!LOADERS && u >= HALF * TM) {
+          if (!LAST || t + STAGES < steps)
+            each<PARTS>([&](auto p) {
+              if constexpr (least(2 * decltype(p)::value, UNITS - HALF * TM - 1) == u - HALF * TM) load(t + STAGES, s, p, last);
+            });
         }
         sums[u % SUMS] = products(ws[Order::slot(i)], xs[j]);
         constexpr int r = Order::reads(u);
