@@ -5,11 +5,13 @@
 // Bound by the bytes: one pass, the row in registers between its sum and its results.  A row is the work of 16 threads up to 128
 // columns (four rows a wave: heads of 128, 81880 rows in 8.4 us, 5.0 TB/s), of a wave up to 512, of 256 threads up to 8192
 // (8192 x 4096 with fp16 residual to 8 bits: 46.9 us, 5.0 TB/s), of 1024 beyond; 8 columns a thread and load.
-// One row (4096 columns) takes 2.4 us on the GPU, of which the host's submission shows 3.5.
+// One row (4096 columns) takes 2.3 us on the GPU, and 3.7 of the host to submit.
 #include "fp8_common.h"
 
 namespace tensor_fp8 {
 namespace {
+
+constexpr int kFewRows = 512;  // two a CU
 
 struct None {};
 struct Codes {};
@@ -101,17 +103,27 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(const NormArgs 
   }
 }
 
-int threads_of(int width) { return width <= 128 ? 16 : width <= 512 ? 64 : width <= 8192 ? 256 : 1024; }
+// Few rows leave CUs idle, so a row is the work of twice the threads or four times, 8 columns each: 64 x 4096 with its fp32
+// residual to 8 bits in 3.3 us (3.7 with 256 threads), 512 x 6144 in 8.3 (10.5), 1 x 5120 in 3.6 (5.1); 1024 x 6144 to fp16
+// would take 11.3 (9.8).
+int threads_of(const NormArgs& a) {
+  const int width = a.width;
+  if (a.rows <= kFewRows && width > 2048 && width <= 8192) return width <= 4096 ? 512 : 1024;
+  return width <= 128 ? 16 : width <= 512 ? 64 : width <= 8192 ? 256 : 1024;
+}
 
 template <typename X, typename R, typename Out>
 hipError_t launch_typed(const NormArgs& a, hipStream_t stream) {
-  const int threads = threads_of(a.width), rows = threads < 256 ? 256 / threads : 1;
+  const int threads = threads_of(a), rows = threads < 256 ? 256 / threads : 1;
   const dim3 grid((unsigned)(((int64_t)a.rows + rows - 1) / rows)), block(threads < 256 ? 256 : threads);
 #define LAUNCH(T, C) hipLaunchKernelGGL((norm_kernel<X, R, Out, T, C>), grid, block, 0, stream, a)
   if (a.width <= 128) LAUNCH(16, 1);
   else if (a.width <= 512) LAUNCH(64, 1);
   else if (a.width <= 2048) LAUNCH(256, 1);
+  else if (threads == 512) LAUNCH(512, 1);
+  else if (threads == 1024 && a.width <= 8192) LAUNCH(1024, 1);
   else if (a.width <= 4096) LAUNCH(256, 2);
+  else if (a.width <= 6144) LAUNCH(256, 3);
   else if (a.width <= 8192) LAUNCH(256, 4);
   else if (a.width <= 16384) LAUNCH(1024, 2);
   else LAUNCH(1024, 4);
@@ -134,7 +146,7 @@ hipError_t launch_residual(const NormArgs& a, hipStream_t stream) {
 }  // namespace
 
 int64_t norm_threads(const NormArgs& a) {
-  const int threads = threads_of(a.width), rows = threads < 256 ? 256 / threads : 1;
+  const int threads = threads_of(a), rows = threads < 256 ? 256 / threads : 1;
   return ((int64_t)a.rows + rows - 1) / rows * (threads < 256 ? 256 : threads);
 }
 

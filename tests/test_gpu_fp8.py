@@ -111,6 +111,20 @@ def test_norm_in_place(hip_device, width):
         assert np.array_equal(xb.to_numpy(), want[0]) and np.array_equal(rb.to_numpy(), want[1])
 
 
+@pytest.mark.parametrize("out", ["float16", "float32", "codes"])
+@pytest.mark.parametrize("width", [2049, 2560, 4096, 4100, 5120, 6144, 6150, 8192])
+def test_norm_of_rows_past_the_few(hip_device, width, out):
+    """512 rows are shared by more threads each than 513."""
+    rng = np.random.default_rng(width)
+    weight = rng.uniform(-1, 2, width).astype(np.float32)
+    for rows, dtype, residual in ((512, "float16", "float16"), (513, "float16", "float32"), (513, "float32", None)):
+        x = (3 * rng.standard_normal((rows, width))).astype(dtype)
+        r = None if residual is None else (5 * rng.standard_normal((rows, width))).astype(residual)
+        x[rows // 2] *= 1e25 if dtype == "float32" else 0  # squares past fp32, or the residual's alone
+        print(f"[case] norm {rows} x {width} {dtype} {residual} {out}", flush=True)
+        check_norm(hip_device, x, r, weight, 1e-6, out)
+
+
 def test_norm_of_many_rows(hip_device):
     rng = np.random.default_rng(0)
     x = rng.standard_normal((70001, 64)).astype(np.float16)
