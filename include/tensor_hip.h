@@ -361,8 +361,8 @@ int32_t tensor_paged_attention_workspace_v1(int64_t tokens, int64_t requests, in
  * What a decoder layer runs around its attention when its linears are held in 8 bits.  No counterpart in the
  * reference.  8 bits are e4m3 (a sign, four bits of exponent with bias 7, three of fraction; no infinities, NaN at 0x7F and
  * 0xFF, values up to 448), in uint8 buffers.  A row of activations has a scale for each 128 columns,
- * s = max(a / 448, 2^-126) with a the largest finite magnitude among them, and the codes nearest to value / s (ties to
- * even; a value that is not finite has the NaN code).  Scales are held [blocks, rows], blocks = ceil(columns / 128).  Rows of
+ * s = max(a / 448, 2^-126) with a the largest finite magnitude among them, and the codes nearest to the quotient value / s in
+ * fp32 (ties to even; a value that is not finite has the NaN code).  Scales are held [blocks, rows], blocks = ceil(columns / 128).  Rows of
  * weights have one for each block of 128 rows x 128 columns.  Buffers are contiguous and 16-byte aligned.  A
  * call refuses a buffer that it writes and that shares memory with another of its buffers, except where it says that the two
  * may be one.

@@ -2,8 +2,8 @@
 //
 // 8 bits are e4m3: a sign, four bits of exponent with bias 7, three of fraction, no infinities, NaN at 0x7F and 0xFF,
 // values up to 448.  A block of 128 columns of a row shares a scale s = max(a / 448, 2^-126), a the largest
-// magnitude of its finite values, and holds the codes nearest to value / s; what is not finite has the NaN code, so that
-// whatever is summed with it is NaN, as it would be without the codes.
+// magnitude of its finite values, and holds the codes nearest to the fp32 quotient value / s, ties to the even one; what is
+// not finite has the NaN code, so that whatever is summed with it is NaN, as it would be without the codes.
 #pragma once
 
 #include "gguf_common.h"
@@ -72,8 +72,17 @@ __device__ __forceinline__ float block_scale(float8_t v, const Chunk& chunk) {
   return fmaxf(top / kLargest, kSmallestScale);
 }
 
-// v / scale as codes, stored
+// v / scale as codes, stored.  q = v (1 / scale) is off by up to 1.5 units of its last place, which turns ties; what it leaves,
+// q scale - v, is exact or a bit short, and taken back times 1 / scale it makes q the quotient but for an error of 2^-22 units.
+// That shows only where the quotient is as near to the middle of two fp32 values, and in a code only where one of the
+// two is a tie of codes: of all scales' and ties' fractions there are 255 such pairs of value and scale, and q is rounded rightly
+// in each.  (What is left of the smallest values would pass below fp32: blocks of small scales are divided 2^64 up.)  An infinite
+// value leaves infinity - infinity, which is the NaN that its code is.
 __device__ __forceinline__ void store_codes(uint8_t* p, float8_t v, float scale, const Chunk& chunk) {
+  if (scale < 0x1p-90f) {
+    scale *= 0x1p64f;
+    v *= 0x1p64f;
+  }
   const float inverse = 1.0f / scale;
   uint32_t words[2];
 #pragma unroll
@@ -82,8 +91,8 @@ __device__ __forceinline__ void store_codes(uint8_t* p, float8_t v, float scale,
     float q[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float size = v[4 * half + e];
-      q[e] = fabsf(size) < kInfinity ? size * inverse : __builtin_nanf("");
+      const float size = v[4 * half + e], near = size * inverse;
+      q[e] = __builtin_fmaf(-__builtin_fmaf(near, scale, -size), inverse, near);
     }
     word = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], word, false);
     word = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], word, true);
