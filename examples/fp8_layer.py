@@ -20,6 +20,7 @@ weights as the codes hold them, without the activations' rounding to 8 bits.
 from __future__ import annotations
 
 import argparse
+import math
 import sys
 from pathlib import Path
 
@@ -142,7 +143,8 @@ def run(*, requests=4, steps=6, hidden=512, inner=1280, heads=8, kv=2, dim=64, p
             histories[b] = torch.cat([histories[b], x[at:at + new].float()])
             want, want_r = formula(layer, histories[b], new)
             for got, exact in ((out, want), (stream, want_r)):
-                worst = max(worst, float((got[at:at + new].double() - exact).norm() / exact.norm()))
+                error = float((got[at:at + new].double() - exact).norm() / exact.norm())
+                worst = max(worst, error if math.isfinite(error) else math.inf)  # (max would pass a NaN by)
             at += new
         print(f"step {step}: {len(y)} tokens, lengths {lengths.tolist()}, {int(layer.left)} pages left, "
               f"largest difference {worst:.4f}", flush=True)

@@ -17,6 +17,7 @@ weights are random; the attention of every token is compared with the formula in
 from __future__ import annotations
 
 import argparse
+import math
 import sys
 from pathlib import Path
 
@@ -124,7 +125,8 @@ def run(*, requests=4, steps=8, prefix=50, hidden=1024, heads=8, kv=2, dim=128, 
         for b, new in enumerate(counts):
             histories[b] = torch.cat([histories[b], x[at:at + new]])
             want, bound = formula(layer, histories[b], new)
-            worst = max(worst, float(((a[at:at + new].double() - want).abs() / bound).max()))
+            error = float(((a[at:at + new].double() - want).abs() / bound).max())
+            worst = max(worst, error if math.isfinite(error) else math.inf)  # (max would pass a NaN by)
             at += new
         print(f"step {step}: {len(x)} tokens, own lengths {lengths.tolist()}, {int(layer.left)} pages left, "
               f"largest difference {worst:.3f} of its bound", flush=True)
