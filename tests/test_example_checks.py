@@ -77,3 +77,10 @@ def test_paged_decode(on_cpu, monkeypatch, value):
     monkeypatch.setattr(paged_decode, "formula", formula)
     worst = paged_decode.run(requests=2, steps=1, prefix=3, hidden=16)
     assert worst == (0.0 if value == 1.0 else 2.0 if value == 1.5 else math.inf)
+
+
+def test_fp8_layer_as_a_program(monkeypatch):
+    """Results that are all zero are off by 1, a part of the layer left out by less: its exit status tells."""
+    for worst, status in ((0.0, 0), (0.2, 0), (0.25, 1), (0.9, 1), (1.0, 1), (math.inf, 1), (math.nan, 1)):
+        monkeypatch.setattr(fp8_layer, "run", lambda **options: worst)
+        assert fp8_layer.main(["--requests", "1"]) == status
