@@ -148,6 +148,8 @@ def quantize_weight(weight) -> tuple:
         raise ValueError("a weight matrix has two dimensions")
     if not np.isfinite(weight).all():
         raise ValueError("weights must be finite")
+    if max(-float(weight.min()), float(weight.max())) / LARGEST > float(np.finfo(np.float32).max):
+        raise ValueError("weights of these magnitudes have no scale in fp32")
     rows, columns = weight.shape
     codes = np.empty(weight.shape, np.uint8)
     scales = np.empty((-(-rows // BLOCK), -(-columns // BLOCK)), np.float32)
