@@ -146,6 +146,8 @@ def quantize_weight(weight) -> tuple:
     weight = np.asarray(weight)
     if weight.ndim != 2 or not weight.size:
         raise ValueError("a weight matrix has two dimensions")
+    if np.iscomplexobj(weight):
+        raise ValueError("weights must be real numbers")
     if not np.isfinite(weight).all():
         raise ValueError("weights must be finite")
     if max(-float(weight.min()), float(weight.max())) / LARGEST > float(np.finfo(np.float32).max):

@@ -28,6 +28,12 @@ def test_magnitudes_up_to_the_largest_scale():
     assert np.allclose(plain.value(codes) * scales.astype(np.float64), weight, rtol=2.0 ** -4)
 
 
+def test_complex_weights_are_refused():
+    """Their imaginary parts would be lost."""
+    with pytest.raises(ValueError, match="real numbers"):
+        fp8.quantize_weight(np.full((2, 2), 1 + 2j))
+
+
 @pytest.mark.parametrize("dtype", ["float16", "float32", "float64", "int8", "int64", "uint8"])
 def test_types_of_real_numbers(dtype):
     weight = np.array([[1, 7], [100, 3]], dtype)
