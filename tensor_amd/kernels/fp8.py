@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import numpy as np
 
-from tensor_amd.kernels.paged import _buffer, _result as _manifest, _scalar
+from tensor_amd.kernels.paged import _buffer, _fp32, _result as _manifest, _scalar
 
 ENTRYPOINTS = {
     "rms_norm": "tensor_rms_norm_v1",
@@ -50,7 +50,7 @@ def _norm(kernel: str, dtype, residual, out_dtype, eps) -> dict:
     dtype = _dtype("dtype", dtype)
     if residual is not None:
         residual = _dtype("residual", residual)
-    if not (isinstance(eps, (int, float)) and not isinstance(eps, bool) and NORM_LEAST_EPS <= np.float32(eps) < np.inf):
+    if not NORM_LEAST_EPS <= _fp32(eps) < np.inf:
         raise ValueError("eps must be a finite number, 2^-100 at least")
     arguments = [_buffer("x", dtype, "M", "D")]
     if residual is not None:

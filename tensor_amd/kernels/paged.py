@@ -110,9 +110,19 @@ def rotary_store_manifest(*, layout: str = "half", dtype="float16") -> dict:
                    shape_divisors={"R": 2}, mutable_inputs=["q_out", "k_cache", "v_cache"])
 
 
+def _fp32(value) -> float:
+    """A number as fp32 holds it, infinite past its largest; NaN for what is no number."""
+    if not isinstance(value, (int, float)) or isinstance(value, bool):
+        return math.nan
+    try:
+        with np.errstate(over="ignore"):
+            return float(np.float32(value))
+    except OverflowError:  # whole numbers past 64-bit floats
+        return math.copysign(math.inf, 1 if value > 0 else -1)
+
+
 def attention_manifest(*, scale: float | None = None) -> dict:
-    if scale is not None and not (isinstance(scale, (int, float)) and not isinstance(scale, bool)
-                                  and 0.0 < np.float32(scale) < np.inf):
+    if scale is not None and not 0.0 < _fp32(scale) < math.inf:
         raise ValueError("scale must be a positive finite number")
     cache = ("N", "G", "L", "D")
     arguments = [
