@@ -402,8 +402,9 @@ int32_t tensor_quantize_fp8_v1(const TensorCallV1 *call, TensorErrorV1 *error);
  *    2 w        uint8 [N, K]                          3 w_scales fp32 [ceil(N / 128), ceil(K / 128)]
  *    4 out      fp16 or fp32 [M, N]
  * fp32 outputs: the codes are widened to fp16 (exactly) and their products added up in fp32.  fp16 outputs: the
- * 8-bit matrix instructions, which within each 8 columns next to each other cut a product off at 2^-13 of the largest power
- * of two there (2 to the sum of a product's two exponents).  M up to 2^20, N 2^22, K 2^20, M N 2^35.
+ * 8-bit matrix instructions, which within each 8 columns next to each other cut a product off, toward zero, at 2^-13 of the largest
+ * power of two there (2 to the sum of a product's two exponents, a code's being -6 below the normal values; products of 0 have none).
+ * Where large products cancel, that may be more than an fp16 rounding of the result.  M up to 2^20, N 2^22, K 2^20, M N 2^35.
  */
 int32_t tensor_fp8_linear_v1(const TensorCallV1 *call, TensorErrorV1 *error);
 
