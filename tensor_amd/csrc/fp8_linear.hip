@@ -10,12 +10,14 @@
 //
 // A step of K is one block, so each 16 x 16 sum of a step is scaled and added once: four vector instructions beside the 32
 // cycles of a product, on a SIMD where they overlap with other products.  What bounds a call:
-//   few rows (linear_rows): the weights' bytes.  1 x 24576 x 4096 in 19.7 us (5.1 TB/s), 16 x 4096 x 12288 in 10.2 (4.9).
+//   few rows (linear_rows): the weights' bytes.  1 x 24576 x 4096 in 19.9 us (5.1 TB/s); 16 x 4096 x 12288 in 10.7 with the weights
+//     in the last cache, 13.2 from memory.
 //   some hundred rows (linear_tiles, 64 x 64 to 256 x 128): a step's chain of LDS reads, products and barrier on the CUs
 //     that have a tile (0.35 us for 128 x 128, of which the products are 0.21), and where weights come from memory a
-//     CU's misses under way.  333 x 6144 x 4096 in 14.7 us (1.14 PFLOP/s) with the weights in the last cache, 20.9 without.
+//     CU's misses under way.  333 x 6144 x 4096 in 15.1 us (1.11 PFLOP/s) with the weights in the last cache, 20.3 without.
 //   thousands (256 x 256): the matrix cores, busy 60% of the cycles, at the clock that their power allows.
-//     8192 x 24576 x 4096 in 680 us (2.42 PFLOP/s; an eighth faster on codes that are all zero).  fp32 results in 1390 us.
+//     8192 x 24576 x 4096 in 684 to 703 us over two runs (2.41 to 2.35 PFLOP/s; an eighth faster on codes that are all zero),
+//     with fp32 results in 1421 us.
 #include <type_traits>
 #include <utility>
 
@@ -119,8 +121,8 @@ struct Units {
 //
 // A wave that loads waits while the CU takes its loads, and so do its products: eight waves of a 128 x 128 tile take 0.42 us a
 // step with loads and 0.33 without.  Four waves that do nothing else leave the others to multiply (0.33 again), one on each
-// SIMD, with larger tiles of their own.  333 x 6144 x 4096 takes 14.7 us, 18.4 without such waves; 2048 x 4096 x 4096
-// takes 30.9 by 256 x 128 tiles with them, 34.1 by 128 x 128 without.  Two waves of 256 x 256 tiles take a SIMD's
+// SIMD, with larger tiles of their own.  When they came, 333 x 6144 x 4096 went from 18.4 us to 14.7, and 2048 x 4096 x 4096
+// from 34.1 by 128 x 128 tiles to 30.9 by 256 x 128.  Two waves of 256 x 256 tiles take a SIMD's
 // registers: no room for a third.
 // Scales come through LDS as well: the wait of a scalar load would wait for every LDS read before it.
 // Prefetches into L2 ahead of the stages, K begun at another block by each workgroup, 32 x 32 x 64 products and more stages were
@@ -281,7 +283,9 @@ __global__ __launch_bounds__(64 * (WN * WM + LOADERS), 2) void linear_tiles(cons
       }
       if constexpr (u < UNITS) {
         constexpr int i = Order::group(u), j = Order::row(u);
-        // one load beside two products (8192 x 24576 x 4096: 676 us, all at once 715)
+        // One load beside two products, as far as there are so many; the others beside the last one.  So, and all at once, in
+        // turn in one run: 256 x 256 at 8192 x 24576 x 4096 701 and 727 us; with fp32 results at 2048 x 4096 x 4096, 128 x 128
+        // 67.3 and 69.2, 128 x 64 78.3 and 79.2; 64 x 64 at 128 x 9728 x 2560 19.5 either way.
         if constexpr (!LOADERS && u >= HALF * TM) {
           if (!LAST || t + STAGES < steps)
             each<PARTS>([&](auto p) {

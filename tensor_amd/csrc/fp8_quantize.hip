@@ -1,8 +1,8 @@
 // Rows as 8-bit codes with a scale for each 128 columns (fp8_common.h): of x, or of silu(g) u for rows [g | u],
 // silu(g) = g / (1 + exp(-g)), in fp32.
 //
-// Bound by the bytes: 16 lanes of 8 columns are a block, which meet in its largest magnitude.  4093 x 12288 gated in 46 us
-// (5.5 TB/s; 61 with rows of blocks one at a time, whose scales lay a row of the scales apart), 8 x 4096 in 2.5 us on the GPU.
+// Bound by the bytes: 16 lanes of 8 columns are a block, which meet in its largest magnitude.  4093 x 12288 gated in 47 us
+// (5.4 TB/s; 61 with rows of blocks one at a time, whose scales lay a row of the scales apart), 8 x 4096 in 2.6 us on the GPU.
 #include "fp8_common.h"
 
 namespace tensor_fp8 {

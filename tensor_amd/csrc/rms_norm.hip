@@ -4,7 +4,8 @@
 //
 // Bound by the bytes: one pass, the row in registers between its sum and its results.  A row is the work of 16 threads up to 128
 // columns (four rows a wave: heads of 128, 81880 rows in 8.4 us, 5.0 TB/s), of a wave up to 512, of 256 threads up to 8192
-// (8192 x 4096 with fp16 residual to 8 bits: 46.9 us, 5.0 TB/s), of 1024 beyond; 8 columns a thread and load.
+// (8192 x 4096 with fp16 residual to 8 bits: 47.3 us, 5.0 TB/s; 512 or 1024 threads where there are few rows), of 1024 beyond; 8
+// columns a thread and load.
 // One row (4096 columns) takes 2.3 us on the GPU, and 3.7 of the host to submit.
 #include "fp8_common.h"
 
@@ -103,9 +104,10 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(const NormArgs 
   }
 }
 
-// Few rows leave CUs idle, so a row is the work of twice the threads or four times, 8 columns each: 64 x 4096 with its fp32
-// residual to 8 bits in 3.3 us (3.7 with 256 threads), 512 x 6144 in 8.3 (10.5), 1 x 5120 in 3.6 (5.1); 1024 x 6144 to fp16
-// would take 11.3 (9.8).
+// Few rows leave CUs idle, so a row is the work of twice the threads or four times, 8 columns each.  By 256 threads and by more, in
+// us: to 8 bits with an fp32 residual 1 x 5120 4.8 and 4.3, 64 x 8192 6.0 and 4.9, 512 x 6144 10.1 and 9.2; to fp16 with an fp16
+// one 1 x 4096 3.1 and 2.9, 512 x 8192 8.4 and 7.8, 512 x 6144 6.9 and 7.1.  The line is where fp16 results lose: 1024 x 6144
+// 9.7 and 11.0.  Results in 8 bits gain past it as well, which it leaves: 600 x 8192 13.7 and 11.8, 8192 x 6144 107.5 and 99.7.
 int threads_of(const NormArgs& a) {
   const int width = a.width;
   if (a.rows <= kFewRows && width > 2048 && width <= 8192) return width <= 4096 ? 512 : 1024;
