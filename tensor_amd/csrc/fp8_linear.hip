@@ -10,14 +10,14 @@
 //
 // A step of K is one block, so each 16 x 16 sum of a step is scaled and added once: four vector instructions beside the 32
 // cycles of a product, on a SIMD where they overlap with other products.  What bounds a call:
-//   few rows (linear_rows): the weights' bytes.  1 x 24576 x 4096 in 19.9 us (5.1 TB/s); 16 x 4096 x 12288 in 10.7 with the weights
-//     in the last cache, 13.2 from memory.
+//   few rows (linear_rows): the weights' bytes.  1 x 24576 x 4096 in 19.9 us (5.1 TB/s); 16 x 4096 x 12288 in 10.2 to 10.7 with the
+//     weights in the last cache, 13.2 from memory.
 //   some hundred rows (linear_tiles, 64 x 64 to 256 x 128): a step's chain of LDS reads, products and barrier on the CUs
 //     that have a tile (0.35 us for 128 x 128, of which the products are 0.21), and where weights come from memory a
-//     CU's misses under way.  333 x 6144 x 4096 in 15.1 us (1.11 PFLOP/s) with the weights in the last cache, 20.3 without.
+//     CU's misses under way.  333 x 6144 x 4096 in 15.2 us (1.10 PFLOP/s) with the weights in the last cache, 20.4 without.
 //   thousands (256 x 256): the matrix cores, busy 60% of the cycles, at the clock that their power allows.
-//     8192 x 24576 x 4096 in 684 to 703 us over two runs (2.41 to 2.35 PFLOP/s; an eighth faster on codes that are all zero),
-//     with fp32 results in 1421 us.
+//     8192 x 24576 x 4096 in 684 to 703 us over four runs (2.41 to 2.35 PFLOP/s; an eighth faster on codes that are all zero),
+//     with fp32 results in 1393 to 1421.
 #include <type_traits>
 #include <utility>
 

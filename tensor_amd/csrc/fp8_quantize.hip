@@ -10,8 +10,12 @@ namespace {
 
 constexpr int kThreads = 256, kLanes = kBlock / 8;  // lanes of a block
 
-// silu(g) v.  Below -80 exp(-g) passes fp32, or what it leaves of the quotient does, while g exp(g) v may not: there
-// exp(g) = m 2^n enters by its exponent, half before and half after v.
+// silu(g) v.  The product that exp takes is rounded once, so a result is off by up to |g| 2^-24 of it where the gate is closed:
+// fp32 inputs by 1 unit of 2^-24 rms from -2 on, by 7 from -20 to -8, by 14 (33 at the most) from -40 to -20, where the gate lets
+// 2^-24 of a value through and less.  A product in two parts would be three instructions a value more.  Of 402 million codes of
+// gated rows 349 differ from those of 64 bits, 371 by a library's exp and quotient in fp32.
+// Below -80 exp(-g) passes fp32, or what it leaves of the quotient does, while g exp(g) v may not: there exp(g) = m 2^n enters by
+// its exponent, half before and half after v.
 __device__ __forceinline__ float8_t gated(float8_t g, float8_t v) {
   constexpr float kLog2 = 1.44269504088896340736f;
   float8_t y;
