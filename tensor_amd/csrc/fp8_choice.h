@@ -11,8 +11,8 @@ namespace tensor_fp8 {
 // them; a round costs `start`, and a step of K `alone` with one workgroup on a CU, `full` with `beside`.  Fitted to calls
 // of 20 to 96 steps and 1 to 4096 rows with weights out of the caches.  There the kernel chosen takes longer than the fastest of
 // them by 0.1% in the mean of 85 calls with fp16 results (3% at the worst) and 0.4% in that of 48 with fp32 ones (20%: 512 x 2500 x
-// 2544 in 21.1 us, 17.6 by 128 x 64 tiles with loaders).  Beyond it, with 4 to 20 steps or weights of 470 MB, it is 1.9% of 40 and
-// 1.5% of 20 calls, 20% at the worst (32 x 57344 x 8192 in 108 us, 90 by 128 x 64 tiles: where the weights' bytes outweigh the
+// 2544 in 21.1 us, 17.6 by 128 x 64 tiles with loaders).  Beyond it, with 4 to 20 steps or weights of 470 MB, it is 2.0% of 40 and
+// 1.4% of 20 calls, 20% at the worst (32 x 57344 x 8192 in 108 us, 90 by 128 x 64 tiles: where the weights' bytes outweigh the
 // estimates, the first of the equal ones is taken).
 struct LinearCost {
   int bn, bm, beside;
